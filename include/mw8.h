@@ -415,6 +415,67 @@ int mw8_moe_prepare_small(const void* logits, int32_t is_bf16, int64_t M, int32_
 int mw8_moe_sum_reduce_bf16(const void* in, int64_t M, int32_t k, int64_t H, void* out,
                             mw8_stream_t stream);
 
+/*
+ * MXFP4 (4-bit e2m1 elements, one E8M0 scale byte per 32 along K; OCP
+ * microscaling).  A quantized matrix [rows, K] is
+ *   codes  uint8 [rows, 16 ceil(K / 32)], two elements per byte, the even
+ *          one in the low half, a last partial block filled with zeros;
+ *   scales uint8 [ceil(K / 512), rows, 16], byte e + 127 of the scale 2^e
+ *          (255: NaN): of the 16 blocks of 512 elements block 8 t + 2 g + s
+ *          is byte 4 g + 2 t + s; bytes of blocks past K must be 0.
+ * Quantizer: e = floor(log2(amax)) - 2 clamped to [-127, 127] (amax = 0: -127),
+ * elements rounded to nearest even, saturating at 6; a block with NaN or an
+ * infinity gets byte 255.  No reference counterpart (the reference has no
+ * quantized path); the entries stand where their int8 namesakes stand.
+ */
+
+/* x bf16 [M, K] (row stride ldx >= K elements, any K) -> q, s.  x 2-byte, q 4-byte aligned
+ * (16-byte loads where x, K and ldx allow). */
+int mw8_quant_mxfp4_bf16(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* q, uint8_t* s,
+                         mw8_stream_t stream);
+
+/* x bf16 [R, 2d] (gate | up) -> q, s of bf16(act(gate) * up) [R, d]; act 0 silu, 1 gelu (erf). */
+int mw8_act_and_mul_quant_mxfp4_bf16(const void* x, int64_t R, int64_t two_d, int32_t act, uint8_t* q, uint8_t* s,
+                                     mw8_stream_t stream);
+
+/* As mw8_rmsnorm_quant_bf16 (residual updated in place, y optional), quantized to q, s; H % 8 == 0, H <= 32768. */
+int mw8_rmsnorm_quant_mxfp4_bf16(const void* x, void* residual, const void* weight, float eps, int64_t M, int64_t H,
+                                 uint8_t* q, uint8_t* s, void* y, mw8_stream_t stream);
+
+/* y bf16 [M, K]: the values that q, s stand for (NaN where a scale byte is 255). */
+int mw8_dequant_mxfp4_bf16(const uint8_t* q, const uint8_t* s, int64_t M, int64_t K, void* y, mw8_stream_t stream);
+
+/*
+ * y bf16 [M, N] = bf16(A W^T + bias[n]), A [M, K] and W [N, K] quantized,
+ * fp32 accumulation.  M >= 0, N and K > 0, K <= 2^20; A, sa, W and sw
+ * 16-byte aligned; bias may be NULL.
+ */
+int mw8_gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias,
+                        void* y, int64_t M, int64_t N, int64_t K, mw8_stream_t stream);
+
+/*
+ * Rotary position embedding of q [T, hq, D] and k [T, hk, D] (token and head
+ * strides ld / hd in elements, heads contiguous) into q_out / k_out (which
+ * may be q / k): pair (a, b) of the first R elements of a head turns to
+ * (a c - b s, b c + a s) with c, s from table fp32 [P, R] (R / 2 cosines,
+ * then R / 2 sines) at the token's position; pairs are (i, R / 2 + i), or
+ * (2 i, 2 i + 1) if interleaved.  q_weight / k_weight [D] (or NULL): per-head
+ * RMSNorm first.  dtype 0 bf16, 1 fp16, 2 fp32; positions int32, or int64 if
+ * pos64; a negative position leaves its rows, one >= P gives NaN.  D <= 8192.
+ * Replaces apply_rope_with_cos_sin_cache_inplace
+ * (python/minisgl/layers/rotary.py:35-52) and the per-head norms before it
+ * (python/minisgl/layers/attention.py:49-53).
+ */
+int mw8_rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int32_t hq, const void* k, int64_t k_ld, int64_t k_hd,
+                  int32_t hk, void* q_out, int64_t qo_ld, int64_t qo_hd, void* k_out, int64_t ko_ld, int64_t ko_hd,
+                  int32_t dtype, int32_t D, int32_t R, int32_t interleaved, const void* positions, int32_t pos64,
+                  const float* table, int64_t P, const void* q_weight, const void* k_weight, float eps, int64_t T,
+                  mw8_stream_t stream);
+
+/* table fp32 [P, 2 pairs]: cos, then sin, of p inv_freq[i] (fp64) times scale. */
+int mw8_rotary_cos_sin(const double* inv_freq, int32_t pairs, int64_t P, double scale, float* table,
+                       mw8_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,6 +73,17 @@ int rmsnorm_strided_bf16(const void*, int64_t, void*, int64_t, const void*, floa
 int linear_bf16_w8a8(const void*, int64_t, const int8_t*, const float*, const void*, void*, int64_t, int64_t,
                      int64_t, hipStream_t);
 int linear_bf16_supported(int64_t, int64_t, int64_t);
+int quant_mxfp4_bf16(const void*, int64_t, int64_t, int64_t, uint8_t*, uint8_t*, hipStream_t);
+int act_and_mul_quant_mxfp4_bf16(const void*, int64_t, int64_t, int, uint8_t*, uint8_t*, hipStream_t);
+int rmsnorm_quant_mxfp4_bf16(const void*, void*, const void*, float, int64_t, int64_t, uint8_t*, uint8_t*, void*,
+                             hipStream_t);
+int dequant_mxfp4_bf16(const uint8_t*, const uint8_t*, int64_t, int64_t, void*, hipStream_t);
+int gemm_mxfp4_bf16(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const void*, void*, int64_t,
+                    int64_t, int64_t, hipStream_t);
+int rotary_qk(const void*, int64_t, int64_t, int, const void*, int64_t, int64_t, int, void*, int64_t, int64_t, void*,
+              int64_t, int64_t, int, int, int, int, const void*, int, const float*, int64_t, const void*, const void*,
+              float, int64_t, hipStream_t);
+int rotary_cos_sin(const double*, int, int64_t, double, float*, hipStream_t);
 
 }  // namespace mw8
 
@@ -264,6 +275,42 @@ int mw8_rmsnorm_quant_bf16(const void* x, void* residual, const void* weight, fl
 int mw8_rmsnorm_strided_bf16(const void* x, int64_t ldx, void* y, int64_t ldy, const void* weight, float eps,
                              int64_t G, int64_t inner, int64_t H, mw8_stream_t st) {
   MW8_ENTRY(mw8::rmsnorm_strided_bf16(x, ldx, y, ldy, weight, eps, G, inner, H, S(st)));
+}
+
+int mw8_quant_mxfp4_bf16(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* q, uint8_t* s, mw8_stream_t st) {
+  MW8_ENTRY(mw8::quant_mxfp4_bf16(x, M, K, ldx, q, s, S(st)));
+}
+
+int mw8_act_and_mul_quant_mxfp4_bf16(const void* x, int64_t R, int64_t two_d, int32_t act, uint8_t* q, uint8_t* s,
+                                     mw8_stream_t st) {
+  MW8_ENTRY(mw8::act_and_mul_quant_mxfp4_bf16(x, R, two_d, act, q, s, S(st)));
+}
+
+int mw8_rmsnorm_quant_mxfp4_bf16(const void* x, void* residual, const void* weight, float eps, int64_t M, int64_t H,
+                                 uint8_t* q, uint8_t* s, void* y, mw8_stream_t st) {
+  MW8_ENTRY(mw8::rmsnorm_quant_mxfp4_bf16(x, residual, weight, eps, M, H, q, s, y, S(st)));
+}
+
+int mw8_dequant_mxfp4_bf16(const uint8_t* q, const uint8_t* s, int64_t M, int64_t K, void* y, mw8_stream_t st) {
+  MW8_ENTRY(mw8::dequant_mxfp4_bf16(q, s, M, K, y, S(st)));
+}
+
+int mw8_gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias,
+                        void* y, int64_t M, int64_t N, int64_t K, mw8_stream_t st) {
+  MW8_ENTRY(mw8::gemm_mxfp4_bf16(A, sa, W, sw, bias, y, M, N, K, S(st)));
+}
+
+int mw8_rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int32_t hq, const void* k, int64_t k_ld, int64_t k_hd,
+                  int32_t hk, void* q_out, int64_t qo_ld, int64_t qo_hd, void* k_out, int64_t ko_ld, int64_t ko_hd,
+                  int32_t dtype, int32_t D, int32_t R, int32_t interleaved, const void* positions, int32_t pos64,
+                  const float* table, int64_t P, const void* q_weight, const void* k_weight, float eps, int64_t T,
+                  mw8_stream_t st) {
+  MW8_ENTRY(mw8::rotary_qk(q, q_ld, q_hd, hq, k, k_ld, k_hd, hk, q_out, qo_ld, qo_hd, k_out, ko_ld, ko_hd, dtype, D, R,
+                           interleaved, positions, pos64, table, P, q_weight, k_weight, eps, T, S(st)));
+}
+
+int mw8_rotary_cos_sin(const double* inv_freq, int32_t pairs, int64_t P, double scale, float* table, mw8_stream_t st) {
+  MW8_ENTRY(mw8::rotary_cos_sin(inv_freq, pairs, P, scale, table, S(st)));
 }
 
 }  // extern "C"

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "mw8_common.h"
+#include "mxfp4.h"
 
 namespace mw8 {
 
@@ -273,7 +274,10 @@ __device__ __forceinline__ double row_sum_f64(double v, double* red) {
 // (r / inner) * ld + (r % inner) * H.  inner = 1, ld = H is a plain [M, H]
 // matrix; a per-head view q.view(M, heads, D) of a row of qkv is inner =
 // heads, ld = qkv width.  residual, q and s are plain [M, H] / [M].
-template <int TPR, int VPT, bool RES, bool QUANT>
+// QUANT: none, per-token int8, or MXFP4 (q and s are then the code and scale
+// bytes of mxfp4.h; a block's four vectors sit in a quad of lanes).
+enum RowQuant : int { kNoQuant = 0, kInt8 = 1, kMxfp4 = 2 };
+template <int TPR, int VPT, bool RES, int QUANT>
 __global__ __launch_bounds__(TPR > 0 ? kBlock : 64 * kMaxWaves) void rmsnorm_rows_kernel(
     const uint16_t* x, uint16_t* __restrict__ res, const uint16_t* __restrict__ w,
     float eps, int64_t M, int64_t H, int8_t* __restrict__ q, float* __restrict__ s,
@@ -333,12 +337,34 @@ __global__ __launch_bounds__(TPR > 0 ? kBlock : 64 * kMaxWaves) void rmsnorm_row
         const float y1 = (bf16_hi(v[i].w[j]) * r) * bf16_hi(wv.w[j]);
         v[i].w[j] = static_cast<uint32_t>(f32_to_bf16(y0)) | (static_cast<uint32_t>(f32_to_bf16(y1)) << 16);
       }
-      if constexpr (QUANT) m = absmax8(v[i], m);
+      if constexpr (QUANT == kInt8) m = absmax8(v[i], m);
     }
   }
-  if constexpr (QUANT) m = row_max<TPR>(m, red);
+  if constexpr (QUANT == kInt8) m = row_max<TPR>(m, red);
   if (!live) return;
-  if constexpr (QUANT) {
+  if constexpr (QUANT == kMxfp4) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    uint8_t* codes = reinterpret_cast<uint8_t*>(q);
+    uint8_t* scales = reinterpret_cast<uint8_t*>(s);
+    const int64_t blocks = mx_blocks(H);
+    auto scale_at = [&](int64_t b) -> uint8_t& {
+      return scales[((b >> 4) * M + row) * kMxTileBlocks + mx_scale_pos(static_cast<int>(b) & 15)];
+    };
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int64_t idx = t + static_cast<int64_t>(i) * tpr;
+      if (idx >= nvec) v[i].w[0] = v[i].w[1] = v[i].w[2] = v[i].w[3] = 0;  // the last block's zeros
+      uint32_t byte;
+      const uint32_t c = mx_quant_quad(v[i], byte);
+      if (idx < 4 * blocks) {
+        reinterpret_cast<uint32_t*>(codes + row * blocks * 16)[idx] = c;
+        if ((t & 3) == 0) scale_at(idx >> 2) = static_cast<uint8_t>(byte);
+      }
+    }
+    for (int64_t b = blocks + t; b < mx_tiles(H) * kMxTileBlocks; b += tpr) scale_at(b) = 0;
+#endif
+  }
+  if constexpr (QUANT == kInt8) {
     const RowScale rs = row_scale(bf16_to_f32(static_cast<uint16_t>(m)));
     uint2* qr = reinterpret_cast<uint2*>(q + row * H);
     if (rs.fast) {
@@ -519,17 +545,32 @@ struct NormLaunch {
                   float eps, int64_t M, int64_t H, int8_t* q, float* s, uint16_t* y, int64_t inner,
                   int64_t ldx, int64_t ldy) {
     if (res && q)
-      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, true, true>), grid, block, 0, st, x, res,
+      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, true, kInt8>), grid, block, 0, st, x, res,
                          w, eps, M, H, q, s, y, inner, ldx, ldy);
     else if (res)
-      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, true, false>), grid, block, 0, st, x, res,
+      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, true, kNoQuant>), grid, block, 0, st, x, res,
                          w, eps, M, H, q, s, y, inner, ldx, ldy);
     else if (q)
-      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, false, true>), grid, block, 0, st, x, res,
+      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, false, kInt8>), grid, block, 0, st, x, res,
                          w, eps, M, H, q, s, y, inner, ldx, ldy);
     else
-      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, false, false>), grid, block, 0, st, x, res,
+      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, false, kNoQuant>), grid, block, 0, st, x, res,
                          w, eps, M, H, q, s, y, inner, ldx, ldy);
+  }
+};
+
+template <int TPR, int VPT>
+struct NormMxLaunch {
+  static void run(dim3 grid, dim3 block, hipStream_t st, const uint16_t* x, uint16_t* res, const uint16_t* w,
+                  float eps, int64_t M, int64_t H, uint8_t* q, uint8_t* s, uint16_t* y) {
+    const auto qi = reinterpret_cast<int8_t*>(q);
+    const auto si = reinterpret_cast<float*>(s);
+    if (res)
+      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, true, kMxfp4>), grid, block, 0, st, x, res,
+                         w, eps, M, H, qi, si, y, int64_t{1}, H, H);
+    else
+      hipLaunchKernelGGL((rmsnorm_rows_kernel<TPR, VPT, false, kMxfp4>), grid, block, 0, st, x, res,
+                         w, eps, M, H, qi, si, y, int64_t{1}, H, H);
   }
 };
 
@@ -595,6 +636,24 @@ int rmsnorm_quant_bf16(const void* x, void* residual, const void* weight, float 
   MW8_REQUIRE(ok, kErrShape, "rmsnorm_quant: H=%lld exceeds the register-resident limit 32768",
               (long long)H);
   return check_launch("rmsnorm_quant");
+}
+
+int rmsnorm_quant_mxfp4_bf16(const void* x, void* residual, const void* weight, float eps, int64_t M, int64_t H,
+                             uint8_t* q, uint8_t* s, void* y, hipStream_t st) {
+  MW8_REQUIRE(x && weight && q && s, kErrArg, "rmsnorm_quant_mxfp4: null pointer");
+  MW8_REQUIRE(M >= 0 && H > 0 && H % 8 == 0, kErrShape, "rmsnorm_quant_mxfp4: need H %% 8 == 0 (H=%lld)",
+              (long long)H);
+  MW8_REQUIRE(eps >= 0.0f, kErrArg, "rmsnorm_quant_mxfp4: eps must be >= 0");
+  if (M == 0) return kOk;
+  MW8_REQUIRE(M < (1ll << 31), kErrShape, "rmsnorm_quant_mxfp4: too many rows");
+  MW8_REQUIRE(aligned16(x) && aligned16(weight) && (reinterpret_cast<uintptr_t>(q) & 3u) == 0 &&
+                  (!residual || aligned16(residual)) && (!y || aligned16(y)),
+              kErrAlign, "rmsnorm_quant_mxfp4: x/residual/weight/y need 16-byte and q 4-byte alignment");
+  const bool ok = dispatch_rows<NormMxLaunch>(RowWork::kNormQuant, H / 8, M, st, static_cast<const uint16_t*>(x),
+                                              static_cast<uint16_t*>(residual), static_cast<const uint16_t*>(weight),
+                                              eps, M, H, q, s, static_cast<uint16_t*>(y));
+  MW8_REQUIRE(ok, kErrShape, "rmsnorm_quant_mxfp4: H=%lld exceeds the register-resident limit 32768", (long long)H);
+  return check_launch("rmsnorm_quant_mxfp4");
 }
 
 int rmsnorm_strided_bf16(const void* x, int64_t ldx, void* y, int64_t ldy, const void* weight, float eps,

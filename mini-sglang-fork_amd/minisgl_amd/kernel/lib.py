@@ -85,6 +85,17 @@ SIGNATURES = {
     ),
     "mw8_rmsnorm_quant_bf16": (ctypes.c_int, [_P, _P, _P, c_float, _I64, _I64, _P, _P, _P, _P]),
     "mw8_rmsnorm_strided_bf16": (ctypes.c_int, [_P, _I64, _P, _I64, _P, c_float, _I64, _I64, _I64, _P]),
+    "mw8_quant_mxfp4_bf16": (ctypes.c_int, [_P, _I64, _I64, _I64, _P, _P, _P]),
+    "mw8_act_and_mul_quant_mxfp4_bf16": (ctypes.c_int, [_P, _I64, _I64, _I32, _P, _P, _P]),
+    "mw8_rmsnorm_quant_mxfp4_bf16": (ctypes.c_int, [_P, _P, _P, c_float, _I64, _I64, _P, _P, _P, _P]),
+    "mw8_dequant_mxfp4_bf16": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _P]),
+    "mw8_gemm_mxfp4_bf16": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "mw8_rotary_qk": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _I32,
+         _P, _I64, _P, _P, c_float, _I64, _P],
+    ),
+    "mw8_rotary_cos_sin": (ctypes.c_int, [_P, _I32, _I64, ctypes.c_double, _P, _P]),
 }
 
 ERROR_NAMES = {

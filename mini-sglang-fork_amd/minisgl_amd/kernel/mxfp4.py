@@ -1,0 +1,230 @@
+"""MXFP4 operators: 4-bit e2m1 elements with one power-of-two scale per 32.
+
+A quantized matrix [rows, K] is two uint8 tensors:
+
+* ``codes`` [rows, 16 * ceil(K / 32)]: two elements per byte, the even one in
+  the low half, a last partial block filled with zeros;
+* ``scale`` [ceil(K / 512), rows, 16]: byte ``e + 127`` of each block's scale
+  2^e (255: NaN), in the order in which the matrix instructions read them:
+  of the 16 blocks of 512 elements, block ``8 t + 2 g + s`` is byte
+  ``4 g + 2 t + s``; bytes of blocks past K are 0.  ``mxfp4_tile_scales``
+  brings the plain [rows, ceil(K / 32)] form into it (a weight's scales,
+  once, when it is loaded), ``mxfp4_row_scales`` back.
+
+Quantization (section 6.3 of the OCP microscaling specification): ``e =
+floor(log2(amax)) - 2`` clamped to [-127, 127], elements rounded to nearest
+even and saturated at 6 * 2^e; a zero block gets byte 0, a block with NaN or
+an infinity byte 255.  Products accumulate in fp32.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .lib import check, load
+from .ops import _ACT, _device_of, _need, _on_gpu, _ptr, _same_device, _stream
+
+
+def _codes_width(K: int) -> int:
+    return (K + 31) // 32 * 16
+
+
+def _tiles(K: int) -> int:
+    return (K + 511) // 512
+
+
+def _empty(rows: int, K: int, like: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    codes = torch.empty((rows, _codes_width(K)), dtype=torch.uint8, device=like.device)
+    scale = torch.empty((_tiles(K), rows, 16), dtype=torch.uint8, device=like.device)
+    return codes, scale
+
+
+def mxfp4_tile_scales(rows: torch.Tensor) -> torch.Tensor:
+    """Scale bytes [rows, blocks] -> the layout [ceil(blocks / 16), rows, 16]
+    of the products (a copy; any device)."""
+    _need(rows.dtype == torch.uint8 and rows.dim() == 2 and rows.shape[1] > 0, "scales: uint8 [rows, blocks]")
+    n, blocks = rows.shape
+    tiles = (blocks + 15) // 16
+    full = torch.zeros((n, tiles * 16), dtype=torch.uint8, device=rows.device)
+    full[:, :blocks].copy_(rows)
+    return full.view(n, tiles, 2, 4, 2).permute(1, 0, 3, 2, 4).reshape(tiles, n, 16)
+
+
+def mxfp4_row_scales(scale: torch.Tensor, K: int) -> torch.Tensor:
+    """The inverse of ``mxfp4_tile_scales``: scale bytes [rows, ceil(K / 32)]."""
+    _need(scale.dtype == torch.uint8 and scale.dim() == 3 and scale.shape[2] == 16 and scale.shape[0] == _tiles(K),
+          "scales: uint8 [ceil(K / 512), rows, 16]")
+    tiles, n, _ = scale.shape
+    rows = scale.view(tiles, n, 4, 2, 2).permute(1, 0, 3, 2, 4).reshape(n, tiles * 16)
+    return rows[:, : (K + 31) // 32].contiguous()
+
+
+def quant_mxfp4(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 [M, K] (any row stride, any K) -> (codes, scale)."""
+    _on_gpu(x)
+    _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[1] > 0, "quant_mxfp4: x must be bf16 [M, K]")
+    _need(x.stride(1) == 1 or x.shape[1] == 1, "quant_mxfp4: last dim must be contiguous")
+    M, K = x.shape
+    _need(M <= 1 or x.stride(0) >= K, "quant_mxfp4: rows must not overlap")
+    codes, scale = _empty(M, K, x)
+    if M > 0:
+        with _device_of(x):
+            check(load().mw8_quant_mxfp4_bf16(_ptr(x), M, K, max(x.stride(0), K), _ptr(codes), _ptr(scale), _stream(x)))
+    return codes, scale
+
+
+def act_and_mul_quant_mxfp4(x: torch.Tensor, activation: str = "silu") -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 [R, 2d] (gate | up) -> (codes, scale) of bf16(act(gate) * up) [R, d]."""
+    _on_gpu(x)
+    _need(activation in _ACT, f"unsupported activation {activation}")
+    _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(), "x: bf16 [R, 2d] contiguous")
+    R, two_d = x.shape
+    _need(two_d > 0 and two_d % 2 == 0, "x: bf16 [R, 2d]")
+    codes, scale = _empty(R, two_d // 2, x)
+    if R > 0:
+        with _device_of(x):
+            check(load().mw8_act_and_mul_quant_mxfp4_bf16(_ptr(x), R, two_d, _ACT[activation], _ptr(codes), _ptr(scale),
+                                                          _stream(x)))
+    return codes, scale
+
+
+def rmsnorm_quant_mxfp4(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float,
+    residual: Optional[torch.Tensor] = None,
+    y: Optional[torch.Tensor] = None,
+    return_y: bool = False,
+):
+    """``rmsnorm_quant`` with the MXFP4 quantizer: bf16 x [M, H] -> (codes,
+    scale[, bf16 y [M, H]]) of the normalized rows, bit-identical to
+    ``quant_mxfp4`` of its y.  ``residual`` is added first and updated in
+    place; ``y`` may be ``x``.  H % 8 == 0, H <= 32768."""
+    _on_gpu(x, weight, residual, y)
+    _same_device(x, weight, residual, y)
+    _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(), "x: bf16 [M, H] contiguous")
+    M, H = x.shape
+    _need(H > 0, "x: bf16 [M, H]")
+    _need(weight.dtype == torch.bfloat16 and weight.shape == (H,) and weight.is_contiguous(), "weight: bf16 [H]")
+    if residual is not None:
+        _need(residual.dtype == torch.bfloat16 and residual.shape == (M, H) and residual.is_contiguous(),
+              "residual: bf16 [M, H] contiguous")
+        _need(M == 0 or residual.data_ptr() != x.data_ptr(), "residual must not be x")
+    if return_y and y is None:
+        y = torch.empty((M, H), dtype=torch.bfloat16, device=x.device)
+    if y is not None:
+        _need(y.dtype == torch.bfloat16 and y.shape == (M, H) and y.is_contiguous(), "y: bf16 [M, H]")
+    codes, scale = _empty(M, H, x)
+    if M > 0:
+        with _device_of(x):
+            check(load().mw8_rmsnorm_quant_mxfp4_bf16(_ptr(x), _ptr(residual), _ptr(weight), float(eps), M, H, _ptr(codes),
+                                                      _ptr(scale), _ptr(y), _stream(x)))
+    return (codes, scale, y) if y is not None else (codes, scale)
+
+
+def _check_operand(name: str, codes: torch.Tensor, scale: torch.Tensor, K: Optional[int]) -> int:
+    """Checks a quantized matrix and returns its rows; K None: a whole number
+    of blocks, as wide as the codes."""
+    _need(codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous() and codes.shape[1] > 0
+          and codes.shape[1] % 16 == 0, f"{name}: codes uint8 [rows, 16 * ceil(K / 32)] contiguous")
+    k = codes.shape[1] * 2 if K is None else K
+    _need(k > 0 and codes.shape[1] == _codes_width(k), f"{name}: codes of {codes.shape[1]} bytes a row do not hold K = {K}")
+    _need(scale.dtype == torch.uint8 and scale.is_contiguous() and scale.shape == (_tiles(k), codes.shape[0], 16),
+          f"{name}: scale uint8 [{_tiles(k)}, {codes.shape[0]}, 16] contiguous (mxfp4_tile_scales)")
+    return codes.shape[0]
+
+
+def dequant_mxfp4(codes: torch.Tensor, scale: torch.Tensor, K: Optional[int] = None) -> torch.Tensor:
+    """The values of a quantized matrix, bf16 [rows, K] (K None: every block whole)."""
+    _on_gpu(codes, scale)
+    _same_device(codes, scale)
+    M = _check_operand("dequant_mxfp4", codes, scale, K)
+    K = codes.shape[1] * 2 if K is None else K
+    y = torch.empty((M, K), dtype=torch.bfloat16, device=codes.device)
+    if M > 0:
+        with _device_of(codes):
+            check(load().mw8_dequant_mxfp4_bf16(_ptr(codes), _ptr(scale), M, K, _ptr(y), _stream(codes)))
+    return y
+
+
+def _check_bias_out(bias, out, M: int, N: int) -> None:
+    if bias is not None:
+        _need(bias.dtype == torch.bfloat16 and bias.shape == (N,) and bias.is_contiguous(), "bias: bf16 [N]")
+    if out is not None:
+        _need(out.dtype == torch.bfloat16 and out.shape == (M, N) and out.is_contiguous(), "out: bf16 [M, N]")
+
+
+def gemm_mxfp4(
+    q: torch.Tensor,
+    s_a: torch.Tensor,
+    w: torch.Tensor,
+    s_w: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """y bf16 [M, N] = bf16(A W^T + bias[n]) of quantized A [M, K], W [N, K]."""
+    _on_gpu(q, s_a, w, s_w, bias, out)
+    _same_device(q, s_a, w, s_w, bias, out)
+    M, N = _check_operand("A", q, s_a, None), _check_operand("W", w, s_w, None)
+    _need(q.shape[1] == w.shape[1], "A/W K mismatch")
+    _need(N > 0, "W: at least one row")
+    _check_bias_out(bias, out, M, N)
+    y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=q.device)
+    if M > 0:
+        with _device_of(q):
+            check(load().mw8_gemm_mxfp4_bf16(_ptr(q), _ptr(s_a), _ptr(w), _ptr(s_w), _ptr(bias), _ptr(y), M, N,
+                                             q.shape[1] * 2, _stream(q)))
+    return y
+
+
+def linear_mxfp4(
+    x: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, bias: Optional[torch.Tensor] = None
+) -> torch.Tensor:
+    """bf16 x [..., K] times a quantized weight [N, K]: y bf16 [..., N].  The
+    rows of x are quantized (``quant_mxfp4``) on the way."""
+    _on_gpu(x, w, s_w, bias)
+    _same_device(x, w, s_w, bias)
+    _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "linear_mxfp4: x must be bf16 [..., K]")
+    N = _check_operand("W", w, s_w, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
+        x2 = x2.contiguous()
+    y = gemm_mxfp4(*quant_mxfp4(x2), w, s_w, bias)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
+def gated_mlp_mxfp4(
+    x: torch.Tensor,
+    w_gate_up: torch.Tensor,
+    s_gate_up: torch.Tensor,
+    w_down: torch.Tensor,
+    s_down: torch.Tensor,
+    activation: str = "silu",
+) -> torch.Tensor:
+    """down(act(gate(x)) * up(x)) on quantized weights gate_up [2I, H] (gate
+    rows first) and down [H', I]: bf16 x [..., H] -> bf16 [..., H'].  gate,
+    up and their product are rounded to bf16 before the product is
+    quantized for down."""
+    _on_gpu(x, w_gate_up, s_gate_up, w_down, s_down)
+    _need(activation in _ACT, f"unsupported activation {activation}")
+    _need(w_gate_up.dim() == 2 and w_gate_up.shape[0] > 0 and w_gate_up.shape[0] % 2 == 0, "w_gate_up: 2I rows")
+    inter = w_gate_up.shape[0] // 2
+    N = _check_operand("down", w_down, s_down, inter)
+    gu = linear_mxfp4(x, w_gate_up, s_gate_up)
+    y = gemm_mxfp4(*act_and_mul_quant_mxfp4(gu.view(-1, 2 * inter), activation), w_down, s_down)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
+__all__ = [
+    "act_and_mul_quant_mxfp4",
+    "dequant_mxfp4",
+    "gated_mlp_mxfp4",
+    "gemm_mxfp4",
+    "linear_mxfp4",
+    "mxfp4_row_scales",
+    "mxfp4_tile_scales",
+    "quant_mxfp4",
+    "rmsnorm_quant_mxfp4",
+]

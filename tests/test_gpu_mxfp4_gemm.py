@@ -1,0 +1,212 @@
+"""GPU parity of the MXFP4 products.  Two kinds of inputs:
+
+* exact: scales 1 and 2, so every product is a multiple of 1/4 and every
+  partial sum, in whatever order, fits fp32's 24 bits (asserted): the result
+  is the exact sum rounded once to bf16, bit for bit;
+* any scale: fp32 sums of K terms, each addition off by at most 2^-23 of the
+  sum of the terms' magnitudes (S), so |y - exact| <= 2^-8 |exact| (the bf16
+  rounding) + (K + 1) 2^-23 S."""
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import announce, f32
+from minisgl_amd.kernel import gated_mlp_mxfp4, gemm_mxfp4, linear_mxfp4, mxfp4_tile_scales, quant_mxfp4
+from oracle import mxfp4 as orc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _operand(rows, K, seed, low=127, high=128):
+    """Random codes and scale bytes in [low, high]: (device pair, fp64 values)."""
+    rng = np.random.default_rng(seed)
+    code = rng.integers(0, 16, (rows, orc.blocks(K) * 32)).astype(np.uint8)
+    code[:, K:] = 0
+    byte = rng.integers(low, high + 1, (rows, orc.blocks(K))).astype(np.uint8)
+    dev = (torch.from_numpy(orc.pack(code)).to(DEV), mxfp4_tile_scales(torch.from_numpy(byte)).to(DEV))
+    return dev, orc.values(code, byte)
+
+
+SIZES = [(1, 16, 32), (1, 1, 32), (1, 5120, 5120), (2, 100, 64), (3, 7168, 1024), (5, 129, 160), (8, 512, 2080),
+         (9, 640, 544), (15, 48, 512), (16, 1000, 5120), (17, 256, 1024), (31, 300, 992), (33, 129, 512), (48, 1024, 768),
+         (64, 2048, 2048), (64, 5120, 1504), (65, 257, 1024), (100, 512, 3200), (127, 640, 256), (128, 768, 5120),
+         (129, 384, 480), (200, 1000, 2048), (256, 256, 256), (257, 520, 1056), (333, 1111, 800), (512, 1024, 1024),
+         (600, 264, 4096), (1025, 768, 288)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("bias", [False, True])
+def test_gemm_exact(M, N, K, bias):
+    announce(f"gemm_mxfp4 exact M={M} N={N} K={K} bias={bias}")
+    a, av = _operand(M, K, seed=M + K)
+    w, wv = _operand(N, K, seed=N * 3 + K)
+    b = np.random.default_rng(N).integers(-8, 9, N) / 4 if bias else None
+    y = gemm_mxfp4(*a, *w, None if b is None else torch.from_numpy(b).bfloat16().to(DEV))
+    want, size = orc.product(av, wv, b)
+    assert size.max() * 4 < 2**24
+    np.testing.assert_array_equal(f32(y).astype(np.float64), orc.round_bf16(want))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 7168, 5120), (7, 333, 1000), (16, 768, 2048), (40, 520, 17408), (130, 512, 5120),
+                                   (300, 1000, 2048)])
+def test_gemm_any_scale(M, N, K):
+    announce(f"gemm_mxfp4 any scale M={M} N={N} K={K}")
+    a, av = _operand(M, K, seed=1, low=110, high=140)
+    w, wv = _operand(N, K, seed=2, low=100, high=130)
+    y = f32(gemm_mxfp4(*a, *w)).astype(np.float64)
+    want, size = orc.product(av, wv)
+    assert (np.abs(y - want) <= 2.0**-8 * np.abs(want) + (K + 1) * 2.0**-23 * size).all()
+
+
+@pytest.mark.parametrize("M", [1, 16, 50, 300])
+def test_gemm_extreme_scales(M):
+    """A NaN scale byte makes its row or column NaN and nothing else; the
+    smallest and largest scales give zeros and infinities without NaN."""
+    announce(f"gemm_mxfp4 extreme scales M={M}")
+    N, K = 300, 1056
+    a, av = _operand(M, K, seed=4)
+    w, wv = _operand(N, K, seed=5)
+    a[1][0, M // 2, 3] = 255
+    w[1][1, 17, 9] = 255
+    y = gemm_mxfp4(*a, *w)
+    nan = torch.isnan(y)
+    want = torch.zeros_like(nan)
+    want[M // 2] = True
+    want[:, 17] = True
+    assert torch.equal(nan, want)
+    a, av = _operand(M, K, seed=6, low=0, high=0)
+    w, wv = _operand(N, K, seed=7, low=20, high=60)
+    assert not gemm_mxfp4(*a, *w).float().abs().gt(1e-30).any()
+    a, _ = _operand(M, K, seed=8, low=254, high=254)
+    w, _ = _operand(N, K, seed=9, low=0, high=0)
+    assert torch.isfinite(gemm_mxfp4(*a, *w).float()).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 5120, 512), (1, 1000, 64), (4, 5120, 7168), (8, 2048, 768), (16, 5120, 640),
+                                   (16, 999, 100), (17, 2048, 768), (100, 520, 264), (333, 5120, 512)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear(M, K, N, bias):
+    """Codes of x are exact, so the only error is the product's."""
+    announce(f"linear_mxfp4 M={M} K={K} N={N} bias={bias}")
+    gen = torch.Generator().manual_seed(M + N)
+    x = torch.randn(M, K, generator=gen).bfloat16()
+    b = torch.randn(N, generator=gen).bfloat16() if bias else None
+    w, wv = _operand(N, K, seed=N, low=110, high=120)
+    y = f32(linear_mxfp4(x.to(DEV), *w, None if b is None else b.to(DEV))).astype(np.float64)
+    want, size = orc.product(orc.values(*orc.quantize(f32(x).astype(np.float64))), wv,
+                             None if b is None else f32(b).astype(np.float64))
+    assert (np.abs(y - want) <= 2.0**-8 * np.abs(want) + (K + 1) * 2.0**-23 * size).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 16])
+def test_linear_layouts(M):
+    """Strided, misaligned and batched rows give the bits of the packed ones."""
+    gen = torch.Generator().manual_seed(M)
+    K, N = 1024, 320
+    w, _ = _operand(N, K, seed=1)
+    x = torch.randn(M, K, generator=gen).bfloat16().to(DEV)
+    want = linear_mxfp4(x, *w)
+    wide = torch.zeros(M, K + 24, dtype=torch.bfloat16, device=DEV)
+    for off in (0, 8, 3):
+        v = wide[:, off : off + K]
+        v.copy_(x)
+        assert torch.equal(linear_mxfp4(v, *w), want)
+    assert torch.equal(linear_mxfp4(x.view(1, M, K), *w), want.view(1, M, N))
+    assert torch.equal(linear_mxfp4(x.t().contiguous().t(), *w), want)
+    assert torch.equal(linear_mxfp4(x[0], *w), want[0])
+    assert torch.equal(gemm_mxfp4(*quant_mxfp4(x), *w), want)
+    x[0, 5] = float("inf")
+    y = linear_mxfp4(x, *w)
+    assert torch.isnan(y[0]).all() and torch.equal(y[1:], want[1:])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,H,I", [(1, 512, 768), (5, 1000, 500), (16, 2048, 768), (70, 512, 640), (300, 1024, 1056),
+                                   (1100, 512, 384)])
+def test_gated_mlp(M, H, I, act):
+    """The chain against itself in fp64.  gate and up are bf16 roundings of
+    fp32 sums, so a sum near a rounding border may round the other way, move
+    the activation by a bf16 step and a code by its spacing: such a code
+    changes h by at most a third of its value (the widest spacing, 4 to 6,
+    is a half of 4 and a third of 6; below 0.5 the value itself is under a
+    quarter of the smallest nonzero level).  Sums of fp32 differ from
+    fp64's by under 2^-20 of S, bf16 borders lie 2^-8 apart and codes change
+    only within 2^-8 of theirs: fewer than 1 in 1000 codes.  The rms of the
+    output moves by less than sqrt(1/1000) / 2 < 2%."""
+    announce(f"gated_mlp_mxfp4 M={M} H={H} I={I} {act}")
+    gen = torch.Generator().manual_seed(M + I)
+    x = torch.randn(M, H, generator=gen).bfloat16()
+    w1, v1 = _operand(2 * I, H, seed=1, low=118, high=121)
+    w2, v2 = _operand(H, I, seed=2, low=118, high=121)
+    y = f32(gated_mlp_mxfp4(x.to(DEV), *w1, *w2, act)).astype(np.float64)
+    gu = orc.round_bf16(orc.product(orc.values(*orc.quantize(f32(x).astype(np.float64))), v1)[0])
+    h = orc.round_bf16(orc.activation(gu[:, :I], act) * gu[:, I:])
+    want = orc.product(orc.values(*orc.quantize(h)), v2)[0]
+    assert np.linalg.norm(y - want) <= 0.02 * np.linalg.norm(want)
+    assert np.isfinite(y).all()
+
+
+def test_gemm_out_and_empty():
+    a, _ = _operand(4, 512, seed=1)
+    w, _ = _operand(40, 512, seed=2)
+    out = torch.full((6, 40), 7.0, dtype=torch.bfloat16, device=DEV)
+    y = gemm_mxfp4(*a, *w, out=out[:4])
+    assert y.data_ptr() == out.data_ptr() and (out[4:] == 7).all()
+    assert torch.equal(y, gemm_mxfp4(*a, *w))
+    e = gemm_mxfp4(a[0][:0], a[1][:, :0].contiguous(), *w)
+    assert e.shape == (0, 40)
+    assert linear_mxfp4(torch.zeros(0, 512, dtype=torch.bfloat16, device=DEV), *w).shape == (0, 40)
+
+
+def test_gemm_refusals():
+    a, _ = _operand(4, 512, seed=1)
+    w, _ = _operand(40, 512, seed=2)
+    v, _ = _operand(40, 544, seed=2)
+    bias = torch.zeros(40, dtype=torch.bfloat16, device=DEV)
+    for call in (
+        lambda: gemm_mxfp4(*a, *v),
+        lambda: gemm_mxfp4(*a, w[0], v[1]),
+        lambda: gemm_mxfp4(a[0].int(), a[1], *w),
+        lambda: gemm_mxfp4(a[0][:, :16], a[1], *w),
+        lambda: gemm_mxfp4(*a, *w, bias=bias.float()),
+        lambda: gemm_mxfp4(*a, *w, bias=bias[:39]),
+        lambda: gemm_mxfp4(*a, *w, bias=bias.cpu()),
+        lambda: gemm_mxfp4(*a, *w, out=torch.zeros(4, 41, dtype=torch.bfloat16, device=DEV)),
+        lambda: linear_mxfp4(torch.zeros(4, 480, dtype=torch.bfloat16, device=DEV), *w),
+        lambda: linear_mxfp4(torch.zeros(4, 512, dtype=torch.float16, device=DEV), *w),
+        lambda: gated_mlp_mxfp4(torch.zeros(4, 512, dtype=torch.bfloat16, device=DEV), *w, *w),
+    ):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("M", [1, 16, 64, 200, 1100])
+def test_streams_and_graph(M):
+    """Eager on the current stream, on a side stream, and captured and replayed
+    with new inputs between eager calls: the same bits."""
+    announce(f"mxfp4 chain on streams and in a graph M={M}")
+    gen = torch.Generator().manual_seed(M)
+    H, I = 1024, 768
+    w1, _ = _operand(2 * I, H, seed=1, low=118, high=121)
+    w2, _ = _operand(H, I, seed=2, low=118, high=121)
+    xs = [torch.randn(M, H, generator=gen).bfloat16().to(DEV) for _ in range(4)]
+    want = [gated_mlp_mxfp4(x, *w1, *w2) for x in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [gated_mlp_mxfp4(x, *w1, *w2) for x in xs]
+    side.synchronize()
+    for g, r in zip(got, want):
+        assert torch.equal(g, r)
+    static = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = gated_mlp_mxfp4(static, *w1, *w2)
+    for i in (1, 2, 3, 0, 1):
+        static.copy_(xs[i])
+        graph.replay()
+        eager = gated_mlp_mxfp4(xs[(i + 1) % 4], *w1, *w2)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i]) and torch.equal(eager, want[(i + 1) % 4])
