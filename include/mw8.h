@@ -448,10 +448,34 @@ int mw8_dequant_mxfp4_bf16(const uint8_t* q, const uint8_t* s, int64_t M, int64_
 /*
  * y bf16 [M, N] = bf16(A W^T + bias[n]), A [M, K] and W [N, K] quantized,
  * fp32 accumulation.  M >= 0, N and K > 0, K <= 2^20; A, sa, W and sw
- * 16-byte aligned; bias may be NULL.
+ * 16-byte aligned; bias may be NULL.  workspace: 16-byte aligned, at least
+ * mw8_gemm_mxfp4_workspace_bytes(M, N, K) bytes (0: none needed), the fp32
+ * sums of a K split; NULL is allowed and only costs speed.  Calls that share
+ * one must be ordered on one stream.
  */
 int mw8_gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias,
-                        void* y, int64_t M, int64_t N, int64_t K, mw8_stream_t stream);
+                        void* y, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                        mw8_stream_t stream);
+size_t mw8_gemm_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+/*
+ * Tiling override of the calling thread's MXFP4 products (cfg 0 ..
+ * mw8_mxfp4_tuning_count() - 1, else automatic; split > 1: K ranges, where
+ * the tiling splits and the workspace allows).  Never changes results beyond
+ * the order of fp32 additions; for tests.
+ */
+void mw8_set_mxfp4_tuning(int32_t cfg, int32_t split);
+int32_t mw8_mxfp4_tuning_count(void);
+
+/*
+ * The quantizer and the product of a decode batch in one launch: x bf16
+ * [M, K] (row stride ldx, 16-byte aligned rows), bit-identical to
+ * mw8_quant_mxfp4_bf16 + mw8_gemm_mxfp4_bf16.  _supported (host only): 1 if
+ * it takes (M, N, K): up to 16 rows, K % 8 == 0, their codes fit a CU's LDS.
+ */
+int mw8_linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_t* sw, const void* bias, void* y,
+                          int64_t M, int64_t N, int64_t K, mw8_stream_t stream);
+int32_t mw8_linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K);
 
 /*
  * Rotary position embedding of q [T, hq, D] and k [T, hk, D] (token and head

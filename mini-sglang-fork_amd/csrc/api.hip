@@ -79,7 +79,13 @@ int rmsnorm_quant_mxfp4_bf16(const void*, void*, const void*, float, int64_t, in
                              hipStream_t);
 int dequant_mxfp4_bf16(const uint8_t*, const uint8_t*, int64_t, int64_t, void*, hipStream_t);
 int gemm_mxfp4_bf16(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const void*, void*, int64_t,
-                    int64_t, int64_t, hipStream_t);
+                    int64_t, int64_t, void*, size_t, hipStream_t);
+size_t gemm_mxfp4_workspace_bytes(int64_t, int64_t, int64_t);
+void set_mxfp4_tuning(int, int);
+int mxfp4_tuning_count();
+int linear_bf16_mxfp4(const void*, int64_t, const uint8_t*, const uint8_t*, const void*, void*, int64_t, int64_t,
+                      int64_t, hipStream_t);
+int linear_bf16_mxfp4_supported(int64_t, int64_t, int64_t);
 int rotary_qk(const void*, int64_t, int64_t, int, const void*, int64_t, int64_t, int, void*, int64_t, int64_t, void*,
               int64_t, int64_t, int, int, int, int, const void*, int, const float*, int64_t, const void*, const void*,
               float, int64_t, hipStream_t);
@@ -296,8 +302,25 @@ int mw8_dequant_mxfp4_bf16(const uint8_t* q, const uint8_t* s, int64_t M, int64_
 }
 
 int mw8_gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias,
-                        void* y, int64_t M, int64_t N, int64_t K, mw8_stream_t st) {
-  MW8_ENTRY(mw8::gemm_mxfp4_bf16(A, sa, W, sw, bias, y, M, N, K, S(st)));
+                        void* y, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, mw8_stream_t st) {
+  MW8_ENTRY(mw8::gemm_mxfp4_bf16(A, sa, W, sw, bias, y, M, N, K, ws, ws_bytes, S(st)));
+}
+
+size_t mw8_gemm_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  return mw8::gemm_mxfp4_workspace_bytes(M, N, K);
+}
+
+void mw8_set_mxfp4_tuning(int32_t cfg, int32_t split) { mw8::set_mxfp4_tuning(cfg, split); }
+
+int32_t mw8_mxfp4_tuning_count(void) { return mw8::mxfp4_tuning_count(); }
+
+int mw8_linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_t* sw, const void* bias, void* y,
+                          int64_t M, int64_t N, int64_t K, mw8_stream_t st) {
+  MW8_ENTRY(mw8::linear_bf16_mxfp4(x, ldx, W, sw, bias, y, M, N, K, S(st)));
+}
+
+int32_t mw8_linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K) {
+  return mw8::linear_bf16_mxfp4_supported(M, N, K);
 }
 
 int mw8_rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int32_t hq, const void* k, int64_t k_ld, int64_t k_hd,

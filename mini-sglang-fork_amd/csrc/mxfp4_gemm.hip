@@ -1,105 +1,242 @@
-// MXFP4 products: y bf16 [M, N] = A W^T of block-scaled 4-bit operands
-// (format: mxfp4.h) on v_mfma_scale_f32_16x16x128_f8f6f4.
-#include <type_traits>
+// MXFP4 products: y bf16 [M, N] = A W^T + bias of block-scaled 4-bit operands
+// (format: mxfp4.h).  Up to 16 tokens stream the weights once
+// (mxfp4_decode.h); more run on tile rings (mxfp4_ring.h), picked by a time
+// model.
+#include <algorithm>
+#include <atomic>
 
-#include "mxfp4.h"
+#include "mxfp4_decode.h"
 
 namespace mw8 {
 
+int device_cus();
+
 namespace {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-struct MxArgs {
-  const uint8_t* A;   // codes [M, 16 Kb]
-  const uint8_t* sa;  // scales [tiles, M, 16]
-  const uint8_t* W;   // codes [N, 16 Kb]
-  const uint8_t* sw;  // scales [tiles, N, 16]
-  const uint16_t* bias;
-  uint16_t* out;
-  int64_t M, N;
-  int kb;     // blocks of 32 along K
-  int tiles;  // 512-element tiles along K
-};
-
-#if defined(__HIP_DEVICE_COMPILE__)
-// D += A B over 128 elements of K; J: the byte of the scale dwords
-template <int J>
-__device__ __forceinline__ v4f mx_mma(v4i a, v4i b, v4f c, int sa, int sb) {
-  const v8i x = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, y = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4 /* e2m1 */, 4, J, sa, J, sb);
-}
-#endif
-
-// One wave per 16 x 64 output tile, fragments straight from global memory.
-__global__ __launch_bounds__(256) void mxfp4_direct_kernel(MxArgs g) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int kFN = 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r16 = lane & 15, grp = lane >> 4;
-  const int64_t m0 = (static_cast<int64_t>(blockIdx.y) * 4 + wave) * 16, n0 = static_cast<int64_t>(blockIdx.x) * 16 * kFN;
-  if (m0 >= g.M) return;
-  const int64_t ld = static_cast<int64_t>(g.kb) * 16;
-  const int64_t am = m0 + r16 < g.M ? m0 + r16 : g.M - 1;
-  const uint8_t* ap = g.A + am * ld;
-  int64_t wn[kFN];
-#pragma unroll
-  for (int j = 0; j < kFN; ++j) wn[j] = n0 + 16 * j + r16 < g.N ? n0 + 16 * j + r16 : g.N - 1;
-  v4f acc[kFN] = {};
-  for (int t = 0; t < g.tiles; ++t) {
-    const int sa = *reinterpret_cast<const int*>(g.sa + (t * g.M + am) * 16 + 4 * grp);
-    int sw[kFN];
-#pragma unroll
-    for (int j = 0; j < kFN; ++j) sw[j] = *reinterpret_cast<const int*>(g.sw + (t * g.N + wn[j]) * 16 + 4 * grp);
-    auto step = [&](auto jc) {
-      constexpr int J = decltype(jc)::value;
-      int c = 16 * t + 8 * (J >> 1) + 2 * grp + (J & 1);
-      c = c < g.kb ? c : g.kb - 1;  // blocks past K: their scales are 2^-127 on both sides
-      const v4i a = *reinterpret_cast<const v4i*>(ap + 16 * c);
-#pragma unroll
-      for (int j = 0; j < kFN; ++j) {
-        const v4i w = *reinterpret_cast<const v4i*>(g.W + wn[j] * ld + 16 * c);
-        acc[j] = mx_mma<J>(a, w, acc[j], sa, sw[j]);
-      }
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 3>{});
-  }
-#pragma unroll
-  for (int j = 0; j < kFN; ++j) {
-    const int64_t n = n0 + 16 * j + r16;
-    if (n >= g.N) continue;
-    const float b = g.bias ? bf16_to_f32(g.bias[n]) : 0.0f;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int64_t m = m0 + 4 * grp + v;
-      if (m < g.M) g.out[m * g.N + n] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(acc[j][v] + b));
-    }
-  }
-#endif
+// Raises the dynamic-LDS limit of kernel Kern once per device (the attribute
+// is set on the current one).
+template <auto Kern>
+int mx_lds_limit(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return set_error(kErrLaunch, "hipGetDevice: %s", hipGetErrorString(e));
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t{1} << dev : 0;
+  if (bit != 0 && (done.load(std::memory_order_acquire) & bit) != 0) return kOk;
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return set_error(kErrLaunch, "hipFuncSetAttribute(%d bytes of LDS): %s", bytes, hipGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_acq_rel);
+  return kOk;
 }
 
 inline bool aligned_to(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+constexpr int kLdsBytes = 163840;
+
+// ------------------------------------------------------------------- rings
+// Tilings and what the time model knows of them (MI355X, fitted to graph-timed
+// runs of 70 random shapes from 17 to 8192 rows): us = start + (rounds - 1)
+// round + max(latency stages rounds, rate stages tiles per CU), at least
+// start + the operands at bw TB/s.  The pick is 2% off the fastest
+// configuration on average, 35% at most (230 x 34816 x 5120).
+struct MxRingCfg {
+  int bm, bn, per_cu;
+  float start, round, latency, rate, bw;
+};
+constexpr MxRingCfg kMxRings[] = {
+    {256, 256, 1, 4.51f, 14.31f, 1.446f, 0.337f, 3.05f},  // 0: a block per CU walks its tiles
+    {256, 192, 1, 3.97f, 9.85f, 1.178f, 0.282f, 2.60f},   // 1: likewise
+    {128, 128, 2, 3.15f, 4.18f, 0.774f, 0.554f, 3.94f},   // 2: likewise, two blocks per CU
+    {128, 128, 1, 4.03f, 4.89f, 0.544f, 0.474f, 4.13f},   // 3: four stages in flight
+    {64, 64, 2, 3.39f, 2.13f, 0.277f, 0.229f, 3.73f},     // 4: likewise; the one that splits K
+};
+constexpr int kNumMxRings = sizeof(kMxRings) / sizeof(kMxRings[0]);
+constexpr int kMxSplitCfg = 4, kMxMaxSplit = 16, kMxDecodeRows = 16;
+
+struct MxPlan {
+  int cfg, split;  // cfg < 0: the decode kernel
+};
+
+thread_local int g_mx_cfg = -1, g_mx_split = 0;  // override of the calling thread (-1: automatic)
+
+double mx_ring_us(int c, int64_t M, int64_t N, int64_t K, int split) {
+  const MxRingCfg& r = kMxRings[c];
+  const int64_t cus = device_cus(), tiles = ((M + r.bm - 1) / r.bm) * ((N + r.bn - 1) / r.bn) * split;
+  const double stages = 2.0 * ((mx_tiles(K) + split - 1) / split);
+  const double rounds = static_cast<double>((tiles + cus * r.per_cu - 1) / (cus * r.per_cu)),
+               per_cu = static_cast<double>((tiles + cus - 1) / cus);
+  double us = r.start + (rounds - 1) * r.round + std::max(r.latency * stages * rounds, r.rate * stages * per_cu);
+  const double bytes = static_cast<double>(N) * K * (17.0 / 32) + 2.0 * M * N;
+  us = std::max(us, r.start + bytes / (r.bw * 1e6));
+  // the sums' way through memory and the second launch
+  if (split > 1) us += 2.3 + 8.0 * split * M * N / 4.4e6;
+  return us;
+}
+
+MxPlan mx_plan(int64_t M, int64_t N, int64_t K, bool may_split) {
+  may_split = may_split && N % 4 == 0;
+  const int64_t tiles = mx_tiles(K);
+  if (g_mx_cfg >= 0) {
+    const bool split = may_split && g_mx_cfg == kMxSplitCfg && g_mx_split > 1 && g_mx_split <= tiles;
+    return {g_mx_cfg, split ? g_mx_split : 1};
+  }
+  if (M <= kMxDecodeRows) return {-1, 1};
+  MxPlan best{0, 1};
+  double us = 1e30;
+  for (int c = 0; c < kNumMxRings; ++c) {
+    const int most = may_split && c == kMxSplitCfg ? static_cast<int>(std::min<int64_t>(kMxMaxSplit, tiles)) : 1;
+    for (int s = 1; s <= most; ++s) {
+      const double t = mx_ring_us(c, M, N, K, s);
+      if (t < us) {
+        us = t;
+        best = {c, s};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BM, int BN, int WM, int WN, int NS, bool kSplit = false>
+int launch_ring(MxArgs g, hipStream_t st) {
+  using R = MxRing<BM, BN, WM, WN, NS>;
+  constexpr auto kern = mxfp4_ring_kernel<BM, BN, WM, WN, NS, kSplit>;
+  constexpr int kThreads = 64 * R::kWaves;
+  const int64_t tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN, slots = device_cus() * (kLdsBytes / R::kLds);
+  MW8_REQUIRE(tm < (1ll << 29) && tn < (1ll << 29) && tm * tn * g.split < (1ll << 31), kErrShape,
+              "gemm_mxfp4: M=%lld x N=%lld too large", (long long)g.M, (long long)g.N);
+  g.raster = MxRaster::of(tm, tn);
+  const int64_t all = tm * tn * g.split, blocks = NS == 2 ? std::min(all, slots) : all;
+  MW8_REQUIRE(blocks * kThreads < (1ll << 32), kErrShape, "gemm_mxfp4: M=%lld x N=%lld too large", (long long)g.M,
+              (long long)g.N);
+  if (const int rc = mx_lds_limit<kern>(R::kLds)) return rc;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), R::kLds, st, g);
+  return check_launch("gemm_mxfp4");
+}
+
+int run_ring(const MxArgs& g, int cfg, hipStream_t st) {
+  switch (cfg) {
+    case 0: return launch_ring<256, 256, 4, 2, 2>(g, st);
+    case 1: return launch_ring<256, 192, 4, 2, 2>(g, st);
+    case 2: return launch_ring<128, 128, 2, 2, 2>(g, st);
+    case 3: return launch_ring<128, 128, 2, 2, 4>(g, st);
+    default: break;
+  }
+  if (g.split == 1) return launch_ring<64, 64, 2, 2, 4>(g, st);
+  if (const int rc = launch_ring<64, 64, 2, 2, 4, true>(g, st)) return rc;
+  const int64_t blocks = (g.M * g.N / 4 + 255) / 256;
+  MW8_REQUIRE(blocks < (1ll << 24), kErrShape, "gemm_mxfp4: M=%lld x N=%lld too large to split", (long long)g.M,
+              (long long)g.N);
+  hipLaunchKernelGGL(mxfp4_split_sum_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, g.part, g.split, g.M,
+                     g.N, g.bias, g.out);
+  return check_launch("gemm_mxfp4");
+}
+
+// ------------------------------------------------------------------ decode
+// 16-row groups per block and 512-element tiles per wave.  Two row groups
+// share the tokens' fragments and leave N <= 32 x CUs one block per CU (MI355X,
+// us, one -> two groups: 16 x 34816 x 5120 24.3 -> 21.7, 16 x 5120 x 17408
+// 15.5 -> 12.8); few tokens and more rows than that are faster in single
+// groups (1 x 34816 x 5120 18.6 -> 17.6, 8 tokens 19.7 -> 19.2).  Four tiles
+// per wave, two where single groups have enough waves (1 x 34816 x 5120 18.3
+// -> 17.6), more where the waves' rings would not fit the LDS.
+struct MxDecodePlan {
+  int groups, per_wave, waves;
+};
+MxDecodePlan mx_decode_plan(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = mx_tiles(K);
+  const int groups = M > 8 || N <= 32 * static_cast<int64_t>(device_cus()) ? 2 : 1;
+  int64_t per = tiles >= 8 ? (groups == 1 ? 2 : 4) : tiles >= 4 ? 2 : 1;
+  const int64_t most = groups == 2 ? 9 : 16, need = (tiles + most - 1) / most;
+  if (per < need) per = need;
+  return {groups, static_cast<int>(per), static_cast<int>((tiles + per - 1) / per)};
+}
+
+constexpr int kMxDepth = 2;  // tiles in flight per wave: 3 or 4 were 5-15% slower (fewer blocks fit the LDS)
+
+int mx_decode_lds(const MxDecodePlan& p, int64_t M, int64_t K, bool xq) {
+  const int ring = p.waves * kMxDepth * p.groups * kMxSlot, sums = p.waves * 16 * (16 * p.groups + 1) * 4;
+  return std::max(ring, sums) + (xq ? static_cast<int>(mx_tiles(K) * M * 272) : 0);
+}
+
+template <int RG, bool kXQ>
+int launch_decode(const MxDecodeArgs& d, const MxDecodePlan& p, hipStream_t st) {
+  constexpr auto kern = mxfp4_decode_kernel<RG, kMxDepth, kXQ>;
+  const int lds = mx_decode_lds(p, d.g.M, d.K, kXQ);
+  if (const int rc = mx_lds_limit<kern>(kLdsBytes)) return rc;
+  const int64_t cus = device_cus(), blocks = cus * ((d.g.N + cus * 16 * RG - 1) / (cus * 16 * RG));
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * p.waves), lds, st, d);
+  return check_launch("gemm_mxfp4");
+}
+
+MxArgs mx_args(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias, void* y,
+               int64_t M, int64_t N, int64_t K) {
+  // (16-byte stores go through a 32-bit view of a tile's output rows)
+  const int store = N % 8 == 0 && aligned_to(y, 16) && N < (1ll << 22) ? 8 : N % 4 == 0 && aligned_to(y, 8) ? 4 : 1;
+  return {A, sa, W, sw, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), M, N,
+          static_cast<int>(mx_blocks(K)), static_cast<int>(mx_tiles(K)), store, {}, nullptr, 1};
+}
+
 }  // namespace
 
+void set_mxfp4_tuning(int cfg, int split) {
+  g_mx_cfg = cfg >= 0 && cfg < kNumMxRings ? cfg : -1;
+  g_mx_split = split;
+}
+int mxfp4_tuning_count() { return kNumMxRings; }
+
+size_t gemm_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const MxPlan p = mx_plan(M, N, K, true);
+  return p.split > 1 ? static_cast<size_t>(p.split) * M * N * 4 : 0;
+}
+
 int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias, void* y,
-                    int64_t M, int64_t N, int64_t K, hipStream_t st) {
+                    int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, hipStream_t st) {
   MW8_REQUIRE(A && sa && W && sw && y, kErrArg, "gemm_mxfp4: null pointer");
   MW8_REQUIRE(M >= 0 && N > 0 && K > 0 && M < (1ll << 31) && N < (1ll << 31) && K <= (1ll << 20), kErrShape,
               "gemm_mxfp4: bad sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
-  MW8_REQUIRE(aligned_to(A, 16) && aligned_to(W, 16) && aligned_to(sa, 16) && aligned_to(sw, 16), kErrAlign,
-              "gemm_mxfp4: A, sa, W and sw need 16-byte alignment");
+  MW8_REQUIRE(aligned_to(A, 16) && aligned_to(W, 16) && aligned_to(sa, 16) && aligned_to(sw, 16) && aligned_to(y, 2) &&
+                  aligned_to(bias, 2) && aligned_to(ws, 16),
+              kErrAlign, "gemm_mxfp4: A, sa, W, sw and the workspace need 16-byte, y and bias 2-byte alignment");
   if (M == 0) return kOk;
-  const MxArgs g{A, sa, W, sw, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), M, N,
-                 static_cast<int>(mx_blocks(K)), static_cast<int>(mx_tiles(K))};
-  const int64_t gy = (M + 63) / 64, gx = (N + 63) / 64;
-  MW8_REQUIRE(gy < 65536, kErrShape, "gemm_mxfp4: M=%lld too large", (long long)M);
-  hipLaunchKernelGGL(mxfp4_direct_kernel, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(256), 0, st, g);
-  return check_launch("gemm_mxfp4");
+  MxArgs g = mx_args(A, sa, W, sw, bias, y, M, N, K);
+  const MxPlan p = mx_plan(M, N, K, ws != nullptr);
+  if (p.cfg < 0) {
+    const MxDecodePlan dp = mx_decode_plan(M, N, K);
+    const MxDecodeArgs d{g, nullptr, 0, K, dp.per_wave};
+    return dp.groups == 2 ? launch_decode<2, false>(d, dp, st) : launch_decode<1, false>(d, dp, st);
+  }
+  if (p.split > 1) {
+    const size_t need = static_cast<size_t>(p.split) * M * N * 4;
+    MW8_REQUIRE(ws_bytes >= need, kErrWorkspace, "gemm_mxfp4: the workspace holds %zu of %zu bytes", ws_bytes, need);
+    g.part = static_cast<float*>(ws);
+    g.split = p.split;
+  }
+  return run_ring(g, p.cfg, st);
+}
+
+// Whether linear_bf16_mxfp4 takes (M, N, K): up to 16 rows whose codes fit
+// the LDS beside the weight ring, K in whole 16-byte vectors.
+int linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || M > kMxDecodeRows || N < 1 || N >= (1ll << 31) || K < 8 || K % 8 != 0 || K > (1ll << 20)) return 0;
+  return g_mx_cfg < 0 && mx_decode_lds(mx_decode_plan(M, N, K), M, K, true) <= kLdsBytes;
+}
+
+int linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_t* sw, const void* bias, void* y, int64_t M,
+                      int64_t N, int64_t K, hipStream_t st) {
+  MW8_REQUIRE(x && W && sw && y, kErrArg, "linear_mxfp4: null pointer");
+  MW8_REQUIRE(M >= 0 && N > 0 && K > 0 && ldx >= K && ldx < (1ll << 26), kErrShape,
+              "linear_mxfp4: bad sizes M=%lld N=%lld K=%lld ldx=%lld", (long long)M, (long long)N, (long long)K, (long long)ldx);
+  if (M == 0) return kOk;
+  MW8_REQUIRE(linear_bf16_mxfp4_supported(M, N, K), kErrShape, "linear_mxfp4: M=%lld N=%lld K=%lld not supported",
+              (long long)M, (long long)N, (long long)K);
+  MW8_REQUIRE(aligned_to(x, 16) && (M == 1 || ldx % 8 == 0) && aligned_to(W, 16) && aligned_to(sw, 16) && aligned_to(y, 2) &&
+                  aligned_to(bias, 2),
+              kErrAlign, "linear_mxfp4: x, its rows, W and sw need 16-byte, y and bias 2-byte alignment");
+  const MxDecodePlan dp = mx_decode_plan(M, N, K);
+  const MxDecodeArgs d{mx_args(nullptr, nullptr, W, sw, bias, y, M, N, K), static_cast<const uint16_t*>(x), ldx, K,
+                       dp.per_wave};
+  return dp.groups == 2 ? launch_decode<2, true>(d, dp, st) : launch_decode<1, true>(d, dp, st);
 }
 
 }  // namespace mw8

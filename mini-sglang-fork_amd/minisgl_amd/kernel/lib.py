@@ -89,7 +89,12 @@ SIGNATURES = {
     "mw8_act_and_mul_quant_mxfp4_bf16": (ctypes.c_int, [_P, _I64, _I64, _I32, _P, _P, _P]),
     "mw8_rmsnorm_quant_mxfp4_bf16": (ctypes.c_int, [_P, _P, _P, c_float, _I64, _I64, _P, _P, _P, _P]),
     "mw8_dequant_mxfp4_bf16": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _P]),
-    "mw8_gemm_mxfp4_bf16": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "mw8_gemm_mxfp4_bf16": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, c_size_t, _P]),
+    "mw8_gemm_mxfp4_workspace_bytes": (c_size_t, [_I64, _I64, _I64]),
+    "mw8_set_mxfp4_tuning": (None, [_I32, _I32]),
+    "mw8_mxfp4_tuning_count": (_I32, []),
+    "mw8_linear_bf16_mxfp4": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "mw8_linear_bf16_mxfp4_supported": (_I32, [_I64, _I64, _I64]),
     "mw8_rotary_qk": (
         ctypes.c_int,
         [_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _I32,

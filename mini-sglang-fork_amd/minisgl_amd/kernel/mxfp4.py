@@ -24,7 +24,7 @@ from typing import Optional, Tuple
 import torch
 
 from .lib import check, load
-from .ops import _ACT, _device_of, _need, _on_gpu, _ptr, _same_device, _stream
+from .ops import _ACT, _call_workspace, _device_of, _need, _on_gpu, _ptr, _same_device, _stream
 
 
 def _codes_width(K: int) -> int:
@@ -174,16 +174,25 @@ def gemm_mxfp4(
     y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=q.device)
     if M > 0:
         with _device_of(q):
-            check(load().mw8_gemm_mxfp4_bf16(_ptr(q), _ptr(s_a), _ptr(w), _ptr(s_w), _ptr(bias), _ptr(y), M, N,
-                                             q.shape[1] * 2, _stream(q)))
+            _gemm(q, s_a, w, s_w, bias, y, M, N)
     return y
+
+
+def _gemm(q, s_a, w, s_w, bias, y, M: int, N: int) -> None:
+    """The product's launch, its tensors checked and their device current."""
+    lib, K = load(), q.shape[1] * 2
+    need = 0 if M <= 16 else lib.mw8_gemm_mxfp4_workspace_bytes(M, N, K)
+    ws = _call_workspace(need, q)
+    check(lib.mw8_gemm_mxfp4_bf16(q.data_ptr(), s_a.data_ptr(), w.data_ptr(), s_w.data_ptr(), _ptr(bias), y.data_ptr(),
+                                  M, N, K, _ptr(ws), need, _stream(q)))
 
 
 def linear_mxfp4(
     x: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, bias: Optional[torch.Tensor] = None
 ) -> torch.Tensor:
     """bf16 x [..., K] times a quantized weight [N, K]: y bf16 [..., N].  The
-    rows of x are quantized (``quant_mxfp4``) on the way."""
+    rows of x are quantized (``quant_mxfp4``) on the way: up to 16 rows
+    inside the product's launch, with the same bits."""
     _on_gpu(x, w, s_w, bias)
     _same_device(x, w, s_w, bias)
     _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "linear_mxfp4: x must be bf16 [..., K]")
@@ -191,6 +200,16 @@ def linear_mxfp4(
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()
+    M, K = x2.shape
+    _check_bias_out(bias, None, M, N)
+    if 0 < M <= 16 and x2.data_ptr() % 16 == 0 and (M == 1 or x2.stride(0) % 8 == 0):
+        lib = load()
+        with _device_of(x):
+            if lib.mw8_linear_bf16_mxfp4_supported(M, N, K):
+                y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+                check(lib.mw8_linear_bf16_mxfp4(x2.data_ptr(), max(x2.stride(0), K), w.data_ptr(), s_w.data_ptr(), _ptr(bias),
+                                                y.data_ptr(), M, N, K, _stream(x)))
+                return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
     y = gemm_mxfp4(*quant_mxfp4(x2), w, s_w, bias)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 

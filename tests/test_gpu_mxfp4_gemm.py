@@ -210,3 +210,77 @@ def test_streams_and_graph(M):
         eager = gated_mlp_mxfp4(xs[(i + 1) % 4], *w1, *w2)
         torch.cuda.synchronize()
         assert torch.equal(y, want[i]) and torch.equal(eager, want[(i + 1) % 4])
+
+
+@pytest.fixture
+def tuning():
+    from minisgl_amd.kernel import load
+
+    lib = load()
+    yield lib.mw8_set_mxfp4_tuning
+    lib.mw8_set_mxfp4_tuning(-1, 0)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 16, 32), (17, 72, 544), (40, 1000, 1024), (130, 252, 2080), (300, 519, 288),
+                                   (513, 1544, 1504), (1100, 1050, 992)])
+@pytest.mark.parametrize("cfg", range(5))
+def test_every_tiling(tuning, cfg, M, N, K):
+    """Every tiling at every size, exact inputs: the automatic choice's bits."""
+    from minisgl_amd.kernel import load
+
+    assert load().mw8_mxfp4_tuning_count() == 5
+    announce(f"gemm_mxfp4 tiling {cfg} M={M} N={N} K={K}")
+    a, av = _operand(M, K, seed=M)
+    w, wv = _operand(N, K, seed=N)
+    b = np.random.default_rng(N).integers(-8, 9, N) / 4
+    tuning(cfg, 0)
+    want, size = orc.product(av, wv, b)
+    assert size.max() * 4 < 2**24
+    bias = torch.from_numpy(b).bfloat16().to(DEV)
+    np.testing.assert_array_equal(f32(gemm_mxfp4(*a, *w, bias)).astype(np.float64), orc.round_bf16(want))
+    # an output whose rows are not 16-byte aligned
+    out = torch.empty(M * N + 1, dtype=torch.bfloat16, device=DEV)[1:].view(M, N)
+    np.testing.assert_array_equal(f32(gemm_mxfp4(*a, *w, bias, out=out)).astype(np.float64), orc.round_bf16(want))
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 64, 1024), (64, 516, 17408), (100, 260, 4128), (65, 1032, 1536)])
+@pytest.mark.parametrize("split", [2, 3, 5, 16])
+def test_split(tuning, split, M, N, K):
+    """K ranges through the workspace: the same bits on exact inputs, twice the
+    same bits on any."""
+    announce(f"gemm_mxfp4 split {split} M={M} N={N} K={K}")
+    a, av = _operand(M, K, seed=M)
+    w, wv = _operand(N, K, seed=N)
+    b = np.random.default_rng(N).integers(-8, 9, N) / 4
+    tuning(4, split)
+    want, _ = orc.product(av, wv, b)
+    y = gemm_mxfp4(*a, *w, torch.from_numpy(b).bfloat16().to(DEV))
+    np.testing.assert_array_equal(f32(y).astype(np.float64), orc.round_bf16(want))
+    a, _ = _operand(M, K, seed=1, low=100, high=150)
+    assert torch.equal(gemm_mxfp4(*a, *w), gemm_mxfp4(*a, *w))
+
+
+def test_workspace():
+    """The size the library asks for, a workspace that is too small, and none."""
+    from minisgl_amd.kernel import load
+    from minisgl_amd.kernel.lib import MW8Error, check
+
+    lib = load()
+    M, N, K = 64, 5120, 17408
+    need = lib.mw8_gemm_mxfp4_workspace_bytes(M, N, K)
+    assert need > 0 and need % (M * N * 4) == 0
+    assert lib.mw8_gemm_mxfp4_workspace_bytes(8192, 34816, 5120) == 0 and lib.mw8_gemm_mxfp4_workspace_bytes(1, N, K) == 0
+    a, av = _operand(M, K, seed=1)
+    w, wv = _operand(N, K, seed=2)
+    want = gemm_mxfp4(*a, *w)
+    y = torch.empty_like(want)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    st = torch.cuda.current_stream().cuda_stream
+    args = (a[0].data_ptr(), a[1].data_ptr(), w[0].data_ptr(), w[1].data_ptr(), None, y.data_ptr(), M, N, K)
+    with pytest.raises(MW8Error, match="WORKSPACE"):
+        check(lib.mw8_gemm_mxfp4_bf16(*args, ws.data_ptr(), need - 1, st))
+    check(lib.mw8_gemm_mxfp4_bf16(*args, ws.data_ptr(), need, st))
+    assert torch.equal(y, want)
+    y.zero_()
+    check(lib.mw8_gemm_mxfp4_bf16(*args, None, 0, st))
+    assert torch.equal(y, want)

@@ -97,11 +97,11 @@ def test_c_refusals():
     assert lib.mw8_dequant_mxfp4_bf16(p, p, 1, 0, p, None) == SHAPE
     assert lib.mw8_dequant_mxfp4_bf16(p, None, 1, 32, p, None) == ARG
     assert lib.mw8_dequant_mxfp4_bf16(odd, p, 1, 32, p, None) == ALIGN
-    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, None, None, p, 1, 16, 32, None) == ARG
-    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, p, None, p, 1, 0, 32, None) == SHAPE
-    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, p, None, p, 1, 16, (1 << 20) + 1, None) == SHAPE
-    assert lib.mw8_gemm_mxfp4_bf16(p, p, odd, p, None, p, 1, 16, 32, None) == ALIGN
-    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, p, None, p, 0, 16, 32, None) == 0
+    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, None, None, p, 1, 16, 32, None, 0, None) == ARG
+    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, p, None, p, 1, 0, 32, None, 0, None) == SHAPE
+    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, p, None, p, 1, 16, (1 << 20) + 1, None, 0, None) == SHAPE
+    assert lib.mw8_gemm_mxfp4_bf16(p, p, odd, p, None, p, 1, 16, 32, None, 0, None) == ALIGN
+    assert lib.mw8_gemm_mxfp4_bf16(p, p, p, p, None, p, 0, 16, 32, None, 0, None) == 0
     assert lib.mw8_last_error()
 
 
