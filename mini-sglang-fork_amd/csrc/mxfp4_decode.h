@@ -15,6 +15,11 @@ struct MxDecodeArgs {
 
 namespace {
 
+// kXQ: rows x tiles that a wave quantizes.  A pass costs a wave some 0.15 us
+// that every block pays: the launch that it saves is worth 8 (MI355X, us,
+// one launch / two: 2 x 5120 -> 7168 7.2 / 8.3, 4 rows 8.7 / 8.4; 4 x 2048 ->
+// 5120 5.1 / 6.3).
+constexpr int kMxPasses = 8;
 constexpr int kMxSlot = 4096;  // 16 weight rows x 256 code bytes (RG of them per tile)
 
 // Block b owns weight rows [N b / G, N (b + 1) / G), at most 16 RG of them,
@@ -115,48 +120,37 @@ __global__ __launch_bounds__(1024) void mxfp4_decode_kernel(MxDecodeArgs d) {
   };
 
   if constexpr (kXQ) {
-    // tokens in passes of one row and tile (8 elements a lane); the first
-    // batch goes out ahead of the weights of the first D tiles, which it is
-    // quantized under
+    // tokens in passes of one row and tile (8 elements a lane), at most
+    // kMxPasses, loaded ahead of the weights of the first D tiles and
+    // quantized under these
     const __amdgpu_buffer_rsrc_t x_rsrc = view(d.x, ((M - 1) * d.ldx + d.K) * 2);
-    constexpr int kBatch = 8;
     const int passes = (t1 - t0) * M;
-    U16x8 v[kBatch];
-    auto load = [&](int p0) {
-      int t = t0 + p0 / M, r = p0 % M;
+    U16x8 v[kMxPasses];
+    int t = t0, r = 0;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int64_t k = static_cast<int64_t>(t) * 512 + 8 * lane;
-        const uint32_t off = p0 + u < passes && k < d.K ? static_cast<uint32_t>((r * d.ldx + k) * 2) : 0x80000000u;
-        const auto q = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, off, 0, 0);
+    for (int u = 0; u < kMxPasses; ++u) {
+      const int64_t k = static_cast<int64_t>(t) * 512 + 8 * lane;
+      const uint32_t off = u < passes && k < d.K ? static_cast<uint32_t>((r * d.ldx + k) * 2) : 0x80000000u;
+      const auto q = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, off, 0, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[u].w[j] = q[j];
-        if (++r == M) {
-          r = 0;
-          ++t;
-        }
+      for (int j = 0; j < 4; ++j) v[u].w[j] = q[j];
+      if (++r == M) {
+        r = 0;
+        ++t;
       }
-    };
-    auto quantize = [&](int p0) {
-      int r = p0 % M;
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (p0 + u >= passes) break;  // wave-uniform
-        uint32_t byte;
-        const uint32_t codes = mx_quant_quad(v[u], byte);
-        unsigned char* row = xq + (p0 + u) * 272;
-        *reinterpret_cast<uint32_t*>(row + 16 * ((lane >> 2) ^ r) + 4 * (lane & 3)) = codes;
-        if ((lane & 3) == 0) row[256 + mx_scale_pos(lane >> 2)] = static_cast<unsigned char>(byte);
-        if (++r == M) r = 0;
-      }
-    };
-    load(0);
+    }
 #pragma unroll
     for (int s = 0; s < D; ++s) issue(s, t0 + s);
-    quantize(0);
-    for (int p0 = kBatch; p0 < passes; p0 += kBatch) {
-      load(p0);
-      quantize(p0);
+    r = 0;
+#pragma unroll
+    for (int u = 0; u < kMxPasses; ++u) {
+      if (u >= passes) break;  // wave-uniform
+      uint32_t byte;
+      const uint32_t codes = mx_quant_quad(v[u], byte);
+      unsigned char* row = xq + u * 272;
+      *reinterpret_cast<uint32_t*>(row + 16 * ((lane >> 2) ^ r) + 4 * (lane & 3)) = codes;
+      if ((lane & 3) == 0) row[256 + mx_scale_pos(lane >> 2)] = static_cast<unsigned char>(byte);
+      if (++r == M) r = 0;
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // this wave's LDS writes (it alone reads them)
   } else {

@@ -215,11 +215,15 @@ int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const
   return run_ring(g, p.cfg, st);
 }
 
-// Whether linear_bf16_mxfp4 takes (M, N, K): up to 16 rows whose codes fit
-// the LDS beside the weight ring, K in whole 16-byte vectors.
+// Whether linear_bf16_mxfp4 takes (M, N, K): few enough rows for each wave's
+// passes (half of them in single row groups, where a CU runs several blocks:
+// 4 x 5120 -> 34816 21.6 us, in two launches 20.4, 2 rows 19.6 and 20.2), their
+// codes beside the weight ring in the LDS, K in whole 16-byte vectors.
 int linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K) {
   if (M < 1 || M > kMxDecodeRows || N < 1 || N >= (1ll << 31) || K < 8 || K % 8 != 0 || K > (1ll << 20)) return 0;
-  return g_mx_cfg < 0 && mx_decode_lds(mx_decode_plan(M, N, K), M, K, true) <= kLdsBytes;
+  const MxDecodePlan p = mx_decode_plan(M, N, K);
+  return g_mx_cfg < 0 && M * p.per_wave <= (p.groups == 2 ? kMxPasses : kMxPasses / 2) &&
+         mx_decode_lds(p, M, K, true) <= kLdsBytes;
 }
 
 int linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_t* sw, const void* bias, void* y, int64_t M,

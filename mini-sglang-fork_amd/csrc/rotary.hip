@@ -16,6 +16,12 @@ namespace {
 // Element types by code (the ABI's dtype argument).
 template <class T> __device__ __forceinline__ float to_f32(T v) { return static_cast<float>(v); }
 
+// 1 / rms of a head, as the row norms compute it: the squares of 24-bit values
+// are exact in fp64, whose sum hides the order that lanes add in.
+__device__ __forceinline__ float norm_factor(double ss, int D, float eps) {
+  return 1.0f / __builtin_sqrtf(static_cast<float>(ss / static_cast<double>(D)) + eps);
+}
+
 struct RotArgs {
   const void* q; const void* k;
   void* q_out; void* k_out;
@@ -49,13 +55,13 @@ __global__ __launch_bounds__(256) void rotary_generic_kernel(RotArgs a) {
   const E* w = static_cast<const E*>(is_q ? a.qw : a.kw);
   float r = 1.0f;
   if (w) {
-    float ss = 0.0f;
+    double ss = 0.0;
     for (int i = lane; i < a.D; i += 64) {
-      const float v = to_f32(x[i]);
-      ss += v * v;
+      const double v = static_cast<double>(to_f32(x[i]));
+      ss = __builtin_fma(v, v, ss);
     }
     for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-    r = 1.0f / __builtin_sqrtf(ss / static_cast<float>(a.D) + a.eps);
+    r = norm_factor(ss, a.D, a.eps);
   }
   auto in = [&](int i) { return w ? to_f32(x[i]) * r * to_f32(w[i]) : to_f32(x[i]); };
   const int half = a.R / 2;
@@ -72,23 +78,164 @@ __global__ __launch_bounds__(256) void rotary_generic_kernel(RotArgs a) {
     for (int i = a.R + lane; i < a.D; i += 64) y[i] = w ? static_cast<E>(in(i)) : x[i];
 }
 
-// table[p, i] = cos(p f_i) * scale, table[p, R/2 + i] = sin(p f_i) * scale,
-// the angle and its functions in fp64.
-__global__ __launch_bounds__(256) void rotary_table_kernel(const double* __restrict__ freq, int half, int64_t P,
-                                                           double scale, float* __restrict__ table) {
-  const int64_t n = P * half, step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < n; e += step) {
-    const int64_t p = e / half;
-    const int i = static_cast<int>(e - p * half);
-    double s, c;
-    sincos(static_cast<double>(p) * freq[i], &s, &c);
-    table[p * 2 * half + i] = static_cast<float>(c * scale);
-    table[p * 2 * half + half + i] = static_cast<float>(s * scale);
+// Whole 16-byte vectors: a lane owns V pairs of a head (V = 8, fp32: 4; two
+// vectors, both halves of its pairs), or 2 V elements past the rotated part;
+// LPH lanes own a head.  A block takes one token and walks its heads, so a
+// lane loads its cosines, sines and norm weights once.  Every element is read
+// and written once; the bound is HBM (MI355X: 8000 tokens x 40 heads of 128,
+// fp16, 64 rotated, @T1@).
+template <class E, bool kInter>
+__global__ __launch_bounds__(1024) void rotary_rows_kernel(RotArgs a, int lph) {
+  constexpr int V = 16 / sizeof(E);
+  struct alignas(16) Vec {
+    E e[V];
+  };
+  const int64_t t = blockIdx.x;
+  const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.pos)[t] : static_cast<const int32_t*>(a.pos)[t];
+  if (p < 0) return;  // a padding token: its rows stay as they are
+  const int u = threadIdx.x & (lph - 1), heads = a.hq + a.hk, slots = blockDim.x / lph;
+  const int half = a.R / 2, turning = half / V;
+  const bool turns = u < turning, live = u < a.D / (2 * V);
+  // the two vectors' first elements
+  const int i0 = kInter || !turns ? 2 * V * u : V * u, i1 = kInter || !turns ? i0 + V : half + V * u;
+  float c[V], s[V];
+  if (live && turns) {
+    const float* cs = a.table + (p < a.P ? p : 0) * a.R + V * u;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      c[j] = cs[j];
+      s[j] = cs[half + j];
+    }
+    if (p >= a.P) {  // past the table
+#pragma unroll
+      for (int j = 0; j < V; ++j) c[j] = s[j] = __builtin_nanf("");
+    }
   }
+  for (int h0 = threadIdx.x / lph; h0 - static_cast<int>(threadIdx.x) / lph < heads; h0 += slots) {
+    const bool on = h0 < heads && live;  // (every lane reaches the shuffles)
+    const bool is_q = h0 < a.hq;
+    const int h = is_q ? h0 : h0 - a.hq;
+    const E* x = is_q ? static_cast<const E*>(a.q) + t * a.q_ld + h * a.q_hd : static_cast<const E*>(a.k) + t * a.k_ld + h * a.k_hd;
+    E* y = is_q ? static_cast<E*>(a.q_out) + t * a.qo_ld + h * a.qo_hd : static_cast<E*>(a.k_out) + t * a.ko_ld + h * a.ko_hd;
+    const E* w = static_cast<const E*>(is_q ? a.qw : a.kw);
+    float f0[V], f1[V];
+    Vec x0{}, x1{};
+    if (on) {
+      x0 = *reinterpret_cast<const Vec*>(x + i0);
+      x1 = *reinterpret_cast<const Vec*>(x + i1);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      f0[j] = to_f32(x0.e[j]);
+      f1[j] = to_f32(x1.e[j]);
+    }
+    if (a.qw || a.kw) {  // launch-uniform
+      double ss = 0.0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        ss = __builtin_fma(static_cast<double>(f0[j]), static_cast<double>(f0[j]), ss);
+        ss = __builtin_fma(static_cast<double>(f1[j]), static_cast<double>(f1[j]), ss);
+      }
+      for (int off = lph / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
+      if (on && w) {
+        const float r = norm_factor(ss, a.D, a.eps);
+        const Vec w0 = *reinterpret_cast<const Vec*>(w + i0), w1 = *reinterpret_cast<const Vec*>(w + i1);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          f0[j] = f0[j] * r * to_f32(w0.e[j]);
+          f1[j] = f1[j] * r * to_f32(w1.e[j]);
+        }
+      }
+    }
+    if (!on || (!turns && !w && x == y)) continue;
+    Vec y0, y1;
+    if (!turns) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        y0.e[j] = w ? static_cast<E>(f0[j]) : x0.e[j];
+        y1.e[j] = w ? static_cast<E>(f1[j]) : x1.e[j];
+      }
+    } else if constexpr (kInter) {
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {  // pairs j of the first vector, V / 2 + j of the second
+        y0.e[2 * j] = static_cast<E>(f0[2 * j] * c[j] - f0[2 * j + 1] * s[j]);
+        y0.e[2 * j + 1] = static_cast<E>(f0[2 * j + 1] * c[j] + f0[2 * j] * s[j]);
+        y1.e[2 * j] = static_cast<E>(f1[2 * j] * c[V / 2 + j] - f1[2 * j + 1] * s[V / 2 + j]);
+        y1.e[2 * j + 1] = static_cast<E>(f1[2 * j + 1] * c[V / 2 + j] + f1[2 * j] * s[V / 2 + j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        y0.e[j] = static_cast<E>(f0[j] * c[j] - f1[j] * s[j]);
+        y1.e[j] = static_cast<E>(f1[j] * c[j] + f0[j] * s[j]);
+      }
+    }
+    *reinterpret_cast<Vec*>(y + i0) = y0;
+    *reinterpret_cast<Vec*>(y + i1) = y1;
+  }
+}
+
+// Sine and cosine of p f in fp64: in turns, whose whole part drops exactly.
+// The error is p f 2^-53, what rounding the product would leave.
+__device__ __forceinline__ void angle_of(double p, double f, double& s, double& c) {
+  const double turn = f * 0.15915494309189535;  // / (2 pi)
+  const double hi = p * turn, lo = __builtin_fma(p, turn, -hi);
+  sincospi(2.0 * ((hi - __builtin_rint(hi)) + lo), &s, &c);
+}
+
+// table[p, i] = cos(p f_i) * scale, table[p, R/2 + i] = sin(p f_i) * scale in
+// fp64.  A thread fills kTableRows positions from two sines: the next angle
+// comes by cos(x + y) = cos x cos y - sin x sin y (the error grows by a few
+// 2^-53 a step), 4 multiplications in place of a sine.  Bound: the stores
+// (MI355X: 131072 x 128 @T2@).
+constexpr int kTableRows = 8;
+__global__ __launch_bounds__(256) void rotary_table_kernel(const double* __restrict__ freq, uint32_t half, int64_t P,
+                                                           double scale, float* __restrict__ table) {
+  const uint32_t n = static_cast<uint32_t>((P + kTableRows - 1) / kTableRows) * half;  // < 2^31 (host)
+  for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
+    const uint32_t q = e / half, i = e - q * half;
+    const int64_t p1 = static_cast<int64_t>(q) * kTableRows;
+    const double f = freq[i];
+    double s, c, s1, c1;
+    angle_of(static_cast<double>(p1), f, s, c);
+    angle_of(1.0, f, s1, c1);
+    float* row = table + p1 * 2 * half + i;
+#pragma unroll
+    for (int r = 0; r < kTableRows; ++r) {
+      if (p1 + r < P) {
+        row[static_cast<int64_t>(2 * r) * half] = static_cast<float>(c * scale);
+        row[static_cast<int64_t>(2 * r + 1) * half] = static_cast<float>(s * scale);
+      }
+      const double cn = __builtin_fma(c, c1, -s * s1);
+      s = __builtin_fma(s, c1, c * s1);
+      c = cn;
+    }
+  }
+}
+
+// Whether every vector of a tensor's rows is 16-byte aligned.
+bool vector_rows(const void* p, int64_t ld, int64_t hd, unsigned size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * size % 16 == 0 && hd * size % 16 == 0;
 }
 
 template <class E>
 int launch_rotary(const RotArgs& a, bool inter, hipStream_t st) {
+  constexpr unsigned size = sizeof(E);
+  constexpr int V = 16 / size;
+  const bool vec = a.R % (2 * V) == 0 && a.D % (2 * V) == 0 && a.D <= 128 * V &&
+                   (a.hq == 0 || (vector_rows(a.q, a.q_ld, a.q_hd, size) && vector_rows(a.q_out, a.qo_ld, a.qo_hd, size))) &&
+                   (a.hk == 0 || (vector_rows(a.k, a.k_ld, a.k_hd, size) && vector_rows(a.k_out, a.ko_ld, a.ko_hd, size))) &&
+                   vector_rows(a.qw, 0, 0, size) && vector_rows(a.kw, 0, 0, size) && vector_rows(a.table, 0, 0, 4);
+  if (vec) {
+    int lph = 1;
+    while (lph < a.D / (2 * V)) lph *= 2;
+    // few tokens: all of a token's heads at once
+    const int most = a.T < 512 ? 1024 : 256, want = (a.hq + a.hk) * lph;
+    const unsigned threads = static_cast<unsigned>(want >= most ? most : (want + 63) / 64 * 64);
+    if (inter) hipLaunchKernelGGL((rotary_rows_kernel<E, true>), dim3(static_cast<unsigned>(a.T)), dim3(threads), 0, st, a, lph);
+    else hipLaunchKernelGGL((rotary_rows_kernel<E, false>), dim3(static_cast<unsigned>(a.T)), dim3(threads), 0, st, a, lph);
+    return check_launch("rotary_qk");
+  }
   const int64_t rows = a.T * (a.hq + a.hk);
   const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
   if (inter) hipLaunchKernelGGL((rotary_generic_kernel<E, true>), dim3(grid), dim3(256), 0, st, a);
@@ -111,7 +258,8 @@ int rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int hq, const void* k, 
   MW8_REQUIRE((hq == 0 || (q && q_out)) && (hk == 0 || (k && k_out)) && pos && table, kErrArg, "rotary_qk: null pointer");
   MW8_REQUIRE(eps >= 0.0f, kErrArg, "rotary_qk: eps must be >= 0");
   if (T == 0) return kOk;
-  MW8_REQUIRE(T < (1ll << 31) / (hq + hk), kErrShape, "rotary_qk: too many rows");
+  // (a launch holds fewer than 2^32 threads, here at most 64 per row or 256 per token)
+  MW8_REQUIRE(T < (1ll << 24) && T < (1ll << 26) / (hq + hk), kErrShape, "rotary_qk: too many rows");
   const unsigned size = dtype == 2 ? 4 : 2;
   auto al = [](const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; };
   MW8_REQUIRE(al(q, size) && al(k, size) && al(q_out, size) && al(k_out, size) && al(table, 4) && al(pos, pos64 ? 8 : 4),
@@ -125,12 +273,12 @@ int rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int hq, const void* k, 
 
 int rotary_cos_sin(const double* freq, int half, int64_t P, double scale, float* table, hipStream_t st) {
   MW8_REQUIRE(freq && table, kErrArg, "rotary_cos_sin: null pointer");
-  MW8_REQUIRE(half > 0 && half <= 4096 && P >= 0 && P < (1ll << 40) / half, kErrShape,
+  MW8_REQUIRE(half > 0 && half <= 4096 && P >= 0 && P < (1ll << 31) / half, kErrShape,
               "rotary_cos_sin: bad sizes P=%lld pairs=%d", (long long)P, half);
   MW8_REQUIRE((reinterpret_cast<uintptr_t>(freq) & 7u) == 0 && (reinterpret_cast<uintptr_t>(table) & 3u) == 0, kErrAlign,
               "rotary_cos_sin: tensors must be aligned to their elements");
   if (P == 0) return kOk;
-  const int64_t blocks = (P * half + 255) / 256;
+  const int64_t blocks = ((P + kTableRows - 1) / kTableRows * half + 255) / 256;
   hipLaunchKernelGGL(rotary_table_kernel, dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st,
                      freq, half, P, scale, table);
   return check_launch("rotary_cos_sin");

@@ -102,8 +102,7 @@ def rmsnorm_quant_mxfp4(
     scale[, bf16 y [M, H]]) of the normalized rows, bit-identical to
     ``quant_mxfp4`` of its y.  ``residual`` is added first and updated in
     place; ``y`` may be ``x``.  H % 8 == 0, H <= 32768."""
-    _on_gpu(x, weight, residual, y)
-    _same_device(x, weight, residual, y)
+    _one_gpu(x, weight, residual, y)
     _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(), "x: bf16 [M, H] contiguous")
     M, H = x.shape
     _need(H > 0, "x: bf16 [M, H]")
@@ -124,22 +123,34 @@ def rmsnorm_quant_mxfp4(
     return (codes, scale, y) if y is not None else (codes, scale)
 
 
+def _one_gpu(*ts: Optional[torch.Tensor]) -> None:
+    """Every tensor on one GPU (``_on_gpu`` and ``_same_device`` in one pass
+    over device indices: an eager decode call is bound by its host time)."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != index or index < 0):
+            _on_gpu(*ts)
+            _same_device(*ts)
+
+
 def _check_operand(name: str, codes: torch.Tensor, scale: torch.Tensor, K: Optional[int]) -> int:
     """Checks a quantized matrix and returns its rows; K None: a whole number
     of blocks, as wide as the codes."""
-    _need(codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous() and codes.shape[1] > 0
-          and codes.shape[1] % 16 == 0, f"{name}: codes uint8 [rows, 16 * ceil(K / 32)] contiguous")
-    k = codes.shape[1] * 2 if K is None else K
-    _need(k > 0 and codes.shape[1] == _codes_width(k), f"{name}: codes of {codes.shape[1]} bytes a row do not hold K = {K}")
-    _need(scale.dtype == torch.uint8 and scale.is_contiguous() and scale.shape == (_tiles(k), codes.shape[0], 16),
-          f"{name}: scale uint8 [{_tiles(k)}, {codes.shape[0]}, 16] contiguous (mxfp4_tile_scales)")
-    return codes.shape[0]
+    if not (codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous() and codes.shape[1] > 0
+            and codes.shape[1] % 16 == 0):
+        raise ValueError(f"{name}: codes uint8 [rows, 16 * ceil(K / 32)] contiguous")
+    rows, width = codes.shape
+    k = width * 2 if K is None else K
+    if not (k > 0 and width == _codes_width(k)):
+        raise ValueError(f"{name}: codes of {width} bytes a row do not hold K = {K}")
+    if not (scale.dtype == torch.uint8 and scale.shape == (_tiles(k), rows, 16) and scale.is_contiguous()):
+        raise ValueError(f"{name}: scale uint8 [{_tiles(k)}, {rows}, 16] contiguous (mxfp4_tile_scales)")
+    return rows
 
 
 def dequant_mxfp4(codes: torch.Tensor, scale: torch.Tensor, K: Optional[int] = None) -> torch.Tensor:
     """The values of a quantized matrix, bf16 [rows, K] (K None: every block whole)."""
-    _on_gpu(codes, scale)
-    _same_device(codes, scale)
+    _one_gpu(codes, scale)
     M = _check_operand("dequant_mxfp4", codes, scale, K)
     K = codes.shape[1] * 2 if K is None else K
     y = torch.empty((M, K), dtype=torch.bfloat16, device=codes.device)
@@ -165,8 +176,7 @@ def gemm_mxfp4(
     out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """y bf16 [M, N] = bf16(A W^T + bias[n]) of quantized A [M, K], W [N, K]."""
-    _on_gpu(q, s_a, w, s_w, bias, out)
-    _same_device(q, s_a, w, s_w, bias, out)
+    _one_gpu(q, s_a, w, s_w, bias, out)
     M, N = _check_operand("A", q, s_a, None), _check_operand("W", w, s_w, None)
     _need(q.shape[1] == w.shape[1], "A/W K mismatch")
     _need(N > 0, "W: at least one row")
@@ -193,8 +203,7 @@ def linear_mxfp4(
     """bf16 x [..., K] times a quantized weight [N, K]: y bf16 [..., N].  The
     rows of x are quantized (``quant_mxfp4``) on the way: up to 16 rows
     inside the product's launch, with the same bits."""
-    _on_gpu(x, w, s_w, bias)
-    _same_device(x, w, s_w, bias)
+    _one_gpu(x, w, s_w, bias)
     _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "linear_mxfp4: x must be bf16 [..., K]")
     N = _check_operand("W", w, s_w, x.shape[-1])
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
@@ -210,7 +219,11 @@ def linear_mxfp4(
                 check(lib.mw8_linear_bf16_mxfp4(x2.data_ptr(), max(x2.stride(0), K), w.data_ptr(), s_w.data_ptr(), _ptr(bias),
                                                 y.data_ptr(), M, N, K, _stream(x)))
                 return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
-    y = gemm_mxfp4(*quant_mxfp4(x2), w, s_w, bias)
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    if M > 0:
+        codes, scale = quant_mxfp4(x2)
+        with _device_of(x):
+            _gemm(codes, scale, w, s_w, bias, y, M, N)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
@@ -226,7 +239,7 @@ def gated_mlp_mxfp4(
     rows first) and down [H', I]: bf16 x [..., H] -> bf16 [..., H'].  gate,
     up and their product are rounded to bf16 before the product is
     quantized for down."""
-    _on_gpu(x, w_gate_up, s_gate_up, w_down, s_down)
+    _one_gpu(x, w_gate_up, s_gate_up, w_down, s_down)
     _need(activation in _ACT, f"unsupported activation {activation}")
     _need(w_gate_up.dim() == 2 and w_gate_up.shape[0] > 0 and w_gate_up.shape[0] % 2 == 0, "w_gate_up: 2I rows")
     inter = w_gate_up.shape[0] // 2

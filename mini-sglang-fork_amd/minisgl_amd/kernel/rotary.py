@@ -9,7 +9,8 @@ from typing import Optional, Tuple
 import torch
 
 from .lib import check, load
-from .ops import _device_of, _need, _on_gpu, _ptr, _same_device, _stream
+from .mxfp4 import _one_gpu
+from .ops import _device_of, _need, _on_gpu, _ptr, _stream
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -17,10 +18,16 @@ _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 def _strides(name: str, t: torch.Tensor) -> Tuple[int, int]:
     """(token, head) strides of t [T, heads, D] with contiguous heads."""
     T, heads, D = t.shape
-    _need(t.stride(2) == 1 or D == 1, f"{name}: last dim must be contiguous")
-    hd = t.stride(1) if heads > 1 else D
-    ld = t.stride(0) if T > 1 else hd * heads
-    _need(hd >= D and (ld >= hd * (heads - 1) + D or hd >= ld * (T - 1) + D), f"{name}: rows must not overlap")
+    ld, hd, one = t.stride()
+    if one != 1 and D != 1:
+        raise ValueError(f"{name}: last dim must be contiguous")
+    if heads <= 1:
+        hd = D
+    if T <= 1:
+        ld = hd * max(heads, 1)
+    # heads within a token's span, or tokens within a head's
+    if not (hd >= D and ld >= hd * (heads - 1) + D or ld >= D and hd >= ld * (T - 1) + D):
+        raise ValueError(f"{name}: rows must not overlap")
     return ld, hd
 
 
@@ -49,8 +56,7 @@ def rotary_qk(
     A token whose position is negative is padding: its output rows stay as
     they are.  One past the table turns to NaN.  Outputs may be the inputs
     themselves; otherwise no output may overlap an input or the other."""
-    _on_gpu(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
-    _same_device(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
+    _one_gpu(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
     _need(q.dtype in _DTYPE and k.dtype == q.dtype, "q and k: bf16, fp16 or fp32, the same")
     _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
           "q: [T, Hq, D] and k: [T, Hk, D]")
@@ -70,10 +76,12 @@ def rotary_qk(
           "q_out and k_out: as q and k")
     if T == 0 or hq + hk == 0:
         return q_out, k_out
+    qs, ks = _strides("q", q), _strides("k", k)
+    qos = qs if q_out is q else _strides("q_out", q_out)
+    kos = ks if k_out is k else _strides("k_out", k_out)
     with _device_of(q):
         check(load().mw8_rotary_qk(
-            _ptr(q), *_strides("q", q), hq, _ptr(k), *_strides("k", k), hk, _ptr(q_out), *_strides("q_out", q_out),
-            _ptr(k_out), *_strides("k_out", k_out), _DTYPE[q.dtype], D, R, int(interleaved), _ptr(positions),
+            _ptr(q), *qs, hq, _ptr(k), *ks, hk, _ptr(q_out), *qos, _ptr(k_out), *kos, _DTYPE[q.dtype], D, R, int(interleaved), _ptr(positions),
             int(positions.dtype == torch.int64), _ptr(cos_sin), P, _ptr(q_weight), _ptr(k_weight), float(eps), T,
             _stream(q)))
     return q_out, k_out
