@@ -86,6 +86,10 @@ int mxfp4_tuning_count();
 int linear_bf16_mxfp4(const void*, int64_t, const uint8_t*, const uint8_t*, const void*, void*, int64_t, int64_t,
                       int64_t, hipStream_t);
 int linear_bf16_mxfp4_supported(int64_t, int64_t, int64_t);
+int gemm_act_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, int, uint8_t*, uint8_t*, int64_t, int64_t,
+                   int64_t, hipStream_t);
+int gemm_act_mxfp4_supported(int64_t, int64_t, int64_t);
+int gemm_act_mxfp4_preferred(int64_t, int64_t, int64_t);
 int rotary_qk(const void*, int64_t, int64_t, int, const void*, int64_t, int64_t, int, void*, int64_t, int64_t, void*,
               int64_t, int64_t, int, int, int, int, const void*, int, const float*, int64_t, const void*, const void*,
               float, int64_t, hipStream_t);
@@ -318,6 +322,15 @@ int mw8_linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const ui
                           int64_t M, int64_t N, int64_t K, mw8_stream_t st) {
   MW8_ENTRY(mw8::linear_bf16_mxfp4(x, ldx, W, sw, bias, y, M, N, K, S(st)));
 }
+
+int mw8_gemm_act_mxfp4(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int32_t act, uint8_t* q,
+                       uint8_t* s, int64_t M, int64_t I, int64_t K, mw8_stream_t st) {
+  MW8_ENTRY(mw8::gemm_act_mxfp4(A, sa, W, sw, act, q, s, M, I, K, S(st)));
+}
+
+int32_t mw8_gemm_act_mxfp4_preferred(int64_t M, int64_t I, int64_t K) { return mw8::gemm_act_mxfp4_preferred(M, I, K); }
+
+int32_t mw8_gemm_act_mxfp4_supported(int64_t M, int64_t I, int64_t K) { return mw8::gemm_act_mxfp4_supported(M, I, K); }
 
 int32_t mw8_linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K) {
   return mw8::linear_bf16_mxfp4_supported(M, N, K);

@@ -96,12 +96,13 @@ MxPlan mx_plan(int64_t M, int64_t N, int64_t K, bool may_split) {
   return best;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool kSplit = false>
+template <int BM, int BN, int WM, int WN, int NS, bool kSplit = false, int kAct = -1>
 int launch_ring(MxArgs g, hipStream_t st) {
   using R = MxRing<BM, BN, WM, WN, NS>;
-  constexpr auto kern = mxfp4_ring_kernel<BM, BN, WM, WN, NS, kSplit>;
+  constexpr auto kern = mxfp4_ring_kernel<BM, BN, WM, WN, NS, kSplit, kAct>;
   constexpr int kThreads = 64 * R::kWaves;
-  const int64_t tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN, slots = device_cus() * (kLdsBytes / R::kLds);
+  const int64_t tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN /* kAct: ceil(I / (BN / 2)) */,
+                slots = device_cus() * (kLdsBytes / R::kLds);
   MW8_REQUIRE(tm < (1ll << 29) && tn < (1ll << 29) && tm * tn * g.split < (1ll << 31), kErrShape,
               "gemm_mxfp4: M=%lld x N=%lld too large", (long long)g.M, (long long)g.N);
   g.raster = MxRaster::of(tm, tn);
@@ -173,7 +174,7 @@ MxArgs mx_args(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint
   // (16-byte stores go through a 32-bit view of a tile's output rows)
   const int store = N % 8 == 0 && aligned_to(y, 16) && N < (1ll << 22) ? 8 : N % 4 == 0 && aligned_to(y, 8) ? 4 : 1;
   return {A, sa, W, sw, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), M, N,
-          static_cast<int>(mx_blocks(K)), static_cast<int>(mx_tiles(K)), store, {}, nullptr, 1};
+          static_cast<int>(mx_blocks(K)), static_cast<int>(mx_tiles(K)), store, {}, nullptr, 1, nullptr, nullptr};
 }
 
 }  // namespace
@@ -213,6 +214,44 @@ int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const
     g.split = p.split;
   }
   return run_ring(g, p.cfg, st);
+}
+
+// Whether gemm_act_mxfp4 takes (M, I, K): whole blocks of activation columns,
+// the weight within a 32-bit view.
+int gemm_act_mxfp4_supported(int64_t M, int64_t I, int64_t K) {
+  return M > 0 && I > 0 && K > 0 && K <= (1ll << 20) && I % kMxBlock == 0 && I < (1ll << 30) &&
+         2 * I * mx_blocks(K) * 16 < (1ll << 31) && M < (1ll << 31);
+}
+
+// Whether it is the faster way to the quantized activation, against the plain
+// product and act_and_mul_quant_mxfp4.  Fused: 6 us, and per round of 256-row x
+// 128-column tiles 3 us + 1.6 us a stage (MI355X, us, fused / two launches: 200 x
+// 25600 x 5120 49 / 69, 2080 rows 294 / 369; 333 x 17408 75 / 63, 2080 rows 193 /
+// 236; 1024 x 6400 39 / 49; K = 2048: 1024 x 768 18 / 13, 8192 rows 22 / 31).
+int gemm_act_mxfp4_preferred(int64_t M, int64_t I, int64_t K) {
+  if (M <= kMxDecodeRows || !gemm_act_mxfp4_supported(M, I, K)) return 0;
+  const int64_t cus = device_cus(), tiles = ((M + 255) / 256) * ((I + 127) / 128);
+  const double rounds = static_cast<double>((tiles + cus - 1) / cus);
+  const double fused = 6.0 + rounds * (3.0 + 1.6 * 2 * mx_tiles(K));
+  double us = 1e30;
+  for (int c = 0; c < kNumMxRings; ++c) us = std::min(us, mx_ring_us(c, M, 2 * I, K, 1));
+  return fused < us + 2.5 + 4.53 * M * I / 5.5e6;
+}
+
+int gemm_act_mxfp4(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int act, uint8_t* q, uint8_t* s,
+                   int64_t M, int64_t I, int64_t K, hipStream_t st) {
+  MW8_REQUIRE(A && sa && W && sw && q && s, kErrArg, "gemm_act_mxfp4: null pointer");
+  MW8_REQUIRE(act == 0 || act == 1, kErrArg, "gemm_act_mxfp4: act must be 0 (silu) or 1 (gelu)");
+  MW8_REQUIRE(M >= 0, kErrShape, "gemm_act_mxfp4: bad size M=%lld", (long long)M);
+  if (M == 0) return kOk;
+  MW8_REQUIRE(gemm_act_mxfp4_supported(M, I, K), kErrShape, "gemm_act_mxfp4: M=%lld I=%lld K=%lld not supported", (long long)M,
+              (long long)I, (long long)K);
+  MW8_REQUIRE(aligned_to(A, 16) && aligned_to(W, 16) && aligned_to(sa, 16) && aligned_to(sw, 16) && aligned_to(q, 8), kErrAlign,
+              "gemm_act_mxfp4: A, sa, W and sw need 16-byte and q 8-byte alignment");
+  MxArgs g = mx_args(A, sa, W, sw, nullptr, nullptr, M, 2 * I, K);
+  g.q = q;
+  g.s = s;
+  return act == 0 ? launch_ring<256, 256, 4, 2, 2, false, 0>(g, st) : launch_ring<256, 256, 4, 2, 2, false, 1>(g, st);
 }
 
 // Whether linear_bf16_mxfp4 takes (M, N, K): few enough rows for each wave's

@@ -61,6 +61,10 @@ struct MxArgs {
   // b % count, p = b / count, and writes fp32 sums to part[p][M][N]
   float* part;
   int split;
+  // kAct kernels: W [2 I, K] holds gate rows, then up rows (N = 2 I); the output
+  // is the quantized activation [M, I]
+  uint8_t* q;
+  uint8_t* s;
 };
 
 namespace {
@@ -99,7 +103,13 @@ struct MxRing {
   static constexpr int kLds = NS * kStage + kScaleSlots * kScale;
 };
 
-template <int BM, int BN, int WM, int WN, int NS, bool kSplit>
+// kAct >= 0 (the activation's code): the tile's weight rows are BN / 2 gate
+// rows and the matching up rows, so that a wave holds both of a column (its
+// first half of fragments gate, its second up).  The epilogue rounds both
+// to bf16, as the plain product stores them, and writes the MXFP4 codes and
+// scales of bf16(act(gate) up): a 32-column fragment is one block per row,
+// shared by lanes l and l + 32.
+template <int BM, int BN, int WM, int WN, int NS, bool kSplit, int kAct>
 __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using R = MxRing<BM, BN, WM, WN, NS>;
@@ -110,10 +120,14 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
   constexpr int kL = kLA + kLB;                          // data DMA instructions per wave and stage
   constexpr int kSUnits = (BM + BN) / 64;                // scale DMA instructions per 512 elements
   constexpr int kLS = (kSUnits + kWaves - 1) / kWaves;   // per wave (the last repeated where it does not divide)
-  constexpr int kStores = kFM * kFN * 2;                 // 16-byte store instructions per wave and tile
+  constexpr int kStores = kAct >= 0 ? kFM * kFN : kFM * kFN * 2;  // store instructions per wave and tile
+  constexpr int kTileN = kAct >= 0 ? BN / 2 : BN;        // output columns of a tile
+  constexpr int kHalf = kWaveN / 2;                      // kAct: gate rows of a wave, and up rows
   constexpr bool kWalk = NS == 2;                        // a block walks tiles blockIdx, blockIdx + gridDim, ...
   static_assert(kLA * 8 * kWaves == BM && kLB * 8 * kWaves == BN && BM % 64 == 0 && BN % 64 == 0, "DMA split");
   static_assert(!kSplit || !kWalk, "a split block owns one tile");
+  static_assert(kAct < 0 || (!kSplit && kHalf == 64), "fused activation: a scale instruction loads one half");
+  const int64_t inter = g.N / 2;  // kAct: rows of each half of W
   static_assert(NS >= 2 && NS <= 4 && R::kLds <= 163840 && kStores + kL + kLS < 64, "ring");
   extern __shared__ __align__(16) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -130,30 +144,55 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
   // The operands of one output tile.  Buffer views of its rows: bytes past
   // the last row read as zeros; those past a row's end read the next row's
   // (their scale bytes are 0 on both sides: the products vanish).
+  // Scale instruction j of this wave fills rows 64 u .. 64 u + 63 of the slot
+  // (the tile's A rows, then its W rows), u = j kWaves + wave; the last is
+  // repeated where waves are left over.
   struct Tile {
     int64_t m0, n0;
-    const uint8_t *a, *w, *sa, *sw;
+    const uint8_t *a, *w;
     int rows_m, rows_n;  // 0: no tile, every load reads zeros
+    const uint8_t* s[kLS];
+    int s_bytes[kLS];
   };
+  int64_t s_step[kLS];  // bytes from one 512 elements' scales to the next
+#pragma unroll
+  for (int j = 0; j < kLS; ++j) {
+    const int u = j * kWaves + wave < kSUnits ? j * kWaves + wave : kSUnits - 1;
+    s_step[j] = (u < BM / 64 ? g.M : g.N) * 16;
+  }
   auto tile_at = [&](uint32_t t) {
     Tile o;
     uint32_t pm, pn;
     const bool live = t < count;
     g.raster.tile(live ? t : 0, pm, pn);
     o.m0 = static_cast<int64_t>(pm) * BM;
-    o.n0 = static_cast<int64_t>(pn) * BN;
+    o.n0 = static_cast<int64_t>(pn) * kTileN;
     o.a = g.A + o.m0 * ld;
     o.w = g.W + o.n0 * ld;
-    o.sa = g.sa + o.m0 * 16;
-    o.sw = g.sw + o.n0 * 16;
     o.rows_m = live ? static_cast<int>(g.M - o.m0 < BM ? g.M - o.m0 : BM) : 0;
-    o.rows_n = live ? static_cast<int>(g.N - o.n0 < BN ? g.N - o.n0 : BN) : 0;
+    // (kAct: every row from the tile's first on, the up rows lie I further)
+    o.rows_n = !live ? 0 : static_cast<int>(kAct >= 0 || g.N - o.n0 < BN ? g.N - o.n0 : BN);
+#pragma unroll
+    for (int j = 0; j < kLS; ++j) {
+      const int u = j * kWaves + wave < kSUnits ? j * kWaves + wave : kSUnits - 1, uw = u - BM / 64;
+      const bool is_a = uw < 0;
+      int64_t row = is_a ? u * 64 : uw * 64;
+      if constexpr (kAct >= 0) row = is_a ? u * 64 : (uw >> 1) * kHalf + (uw & 1) * inter;
+      const int64_t left = (is_a ? o.rows_m : o.rows_n) - row;
+      o.s[j] = (is_a ? g.sa + (kt0 * g.M + o.m0) * 16 : g.sw + (kt0 * g.N + o.n0) * 16) + row * 16;
+      o.s_bytes[j] = __builtin_amdgcn_readfirstlane(static_cast<int>(left < 0 ? 0 : left < 64 ? left * 16 : 1024));
+    }
     return o;
   };
   // field by field (a choice between two references would put both in memory)
   auto pick = [](bool c, const Tile& x, const Tile& y) {
-    return Tile{c ? x.m0 : y.m0, c ? x.n0 : y.n0,         c ? x.a : y.a,          c ? x.w : y.w,
-                c ? x.sa : y.sa, c ? x.sw : y.sw, c ? x.rows_m : y.rows_m, c ? x.rows_n : y.rows_n};
+    Tile o{c ? x.m0 : y.m0, c ? x.n0 : y.n0, c ? x.a : y.a, c ? x.w : y.w, c ? x.rows_m : y.rows_m, c ? x.rows_n : y.rows_n, {}, {}};
+#pragma unroll
+    for (int j = 0; j < kLS; ++j) {
+      o.s[j] = c ? x.s[j] : y.s[j];
+      o.s_bytes[j] = c ? x.s_bytes[j] : y.s_bytes[j];
+    }
+    return o;
   };
   auto view = [](const uint8_t* p, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(scalar_ptr(const_cast<uint8_t*>(p)), 0,
@@ -169,7 +208,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
 #pragma unroll
   for (int j = 0; j < kLB; ++j) {
     const int unit = (j * kWaves + wave) * 64 + lane, row = unit >> 3;
-    w_off[j] = static_cast<uint32_t>(row * ld + 16 * ((unit & 7) ^ swz_f<128>(row)));
+    int64_t at = row;  // the tile row's row of W from the tile's first
+    if constexpr (kAct >= 0) at = row / kWaveN * kHalf + row % kHalf + (row % kWaveN < kHalf ? 0 : inter);
+    w_off[j] = static_cast<uint32_t>(at * ld + 16 * ((unit & 7) ^ swz_f<128>(row)));
   }
   auto issue_data = [&](const Tile& o, int slot, int s) {
     unsigned char* base = lds + slot * R::kStage;
@@ -183,20 +224,14 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr_t)(base + R::kStageA + (j * kWaves + wave) * 1024), 16, w_off[j],
                                                k0, 0, 0);
   };
-  // scales of the tile's 512 elements number p: instruction u fills rows
-  // 64 u .. 64 u + 63 of the slot (the tile's A rows, then its W rows)
+  // scales of the tile's 512 elements number p
   auto issue_scales = [&](const Tile& o, int slot, int p) {
-    const int64_t t = kt0 + p;
     unsigned char* base = lds + NS * R::kStage + slot * R::kScale;
 #pragma unroll
     for (int j = 0; j < kLS; ++j) {
       const int u = j * kWaves + wave < kSUnits ? j * kWaves + wave : kSUnits - 1;
-      const bool is_a = u < BM / 64;
-      const int row = (is_a ? u : u - BM / 64) * 64;
-      const int rows = is_a ? o.rows_m : o.rows_n;
-      const __amdgpu_buffer_rsrc_t rs =
-          view(is_a ? o.sa + t * g.M * 16 : o.sw + t * g.N * 16, rows * 16);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(base + u * 1024), 16, row * 16 + lane * 16, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(view(o.s[j] + p * s_step[j], o.s_bytes[j]), (lds_ptr_t)(base + u * 1024), 16,
+                                               lane * 16, 0, 0, 0);
     }
   };
 
@@ -292,6 +327,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
   Tile none = cur;
   none.rows_m = none.rows_n = 0;
 #pragma unroll
+  for (int j = 0; j < kLS; ++j) none.s_bytes[j] = 0;
+#pragma unroll
   for (int s = 0; s < NS; ++s) {
     const Tile from = pick(s < ns, cur, none);
     const int at = s < ns ? s : 0;
@@ -319,7 +356,58 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
     // ---- epilogue: lane holds columns 32 j + 8 b + 4 grp + v of row 32 i + r32
     const int64_t mw = cur.m0 + wm * kWaveM, nw = cur.n0 + wn * kWaveN;
     auto bias_of = [&](int64_t n) { return g.bias && n < g.N ? bf16_to_f32(g.bias[n]) : 0.0f; };
-    if constexpr (kSplit) {
+    if constexpr (kAct >= 0) {
+      const int64_t ldq = inter / 2;  // I % 32 == 0 (host)
+      const int last = static_cast<int>(mx_tiles(inter)) * kMxTileBlocks, blocks = static_cast<int>(inter / kMxBlock);
+      const int64_t cw = cur.n0 + wn * kHalf;  // the wave's first column
+      if (cur.n0 + kTileN >= inter && wn == WN - 1) {  // the bytes of blocks past I (beyond the counted stores)
+        for (int b = blocks; b < last; ++b)
+#pragma unroll
+          for (int i = 0; i < kFM; ++i) {
+            const int64_t m = mw + 32 * i + r32;
+            if (grp == 0 && m < g.M) g.s[((b >> 4) * g.M + m) * kMxTileBlocks + mx_scale_pos(b & 15)] = 0;
+          }
+      }
+      const __amdgpu_buffer_rsrc_t rq = view(g.q + cur.m0 * ldq, cur.rows_m * ldq);
+#pragma unroll
+      for (int j = 0; j < kFN / 2; ++j) {
+        const int64_t c = cw + 32 * j;
+        const bool in = c < inter;  // whole blocks
+        const int b = in ? static_cast<int>(c / kMxBlock) : 0;
+        const __amdgpu_buffer_rsrc_t rs =
+            view(g.s + ((b >> 4) * g.M + cur.m0) * kMxTileBlocks, in ? cur.rows_m * kMxTileBlocks : 0);
+#pragma unroll
+        for (int i = 0; i < kFM; ++i) {
+          U16x8 lo, hi;  // columns 8 b + 4 grp + v, b = 0, 1 and b = 2, 3
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            float a[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float gate = static_cast<float>(static_cast<__bf16>(acc[i][j][2 * v + k]));
+              const float up = static_cast<float>(static_cast<__bf16>(acc[i][j + kFN / 2][2 * v + k]));
+              a[k] = act_fn<kAct>(gate) * up;
+            }
+            const mx_bf16x2 p = {static_cast<__bf16>(a[0]), static_cast<__bf16>(a[1])};
+            (v < 4 ? lo.w[v] : hi.w[v - 4]) = __builtin_bit_cast(uint32_t, p);
+          }
+          const uint32_t mine = mx_absmax8(lo), rest = mx_absmax8(hi), most = mine > rest ? mine : rest;
+          const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+          const uint32_t byte = mx_scale_byte(both[0] > both[1] ? both[0] : both[1]);
+          const float scale = mx_scale_value(byte == 255u ? 0u : byte);
+          const uint32_t c01 = byte == 255u ? 0u : mx_codes8(lo, scale), c23 = byte == 255u ? 0u : mx_codes8(hi, scale);
+          // lane l takes both lanes' codes of b = 0, 1, lane l + 32 those of b = 2, 3
+          const auto x = __builtin_amdgcn_permlane32_swap(c01, c23, false, false);
+          const int row = wm * kWaveM + 32 * i + r32;
+          typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+          const u32x2 codes = {(x[0] & 0xFFFFu) | (x[1] << 16), (x[0] >> 16) | (x[1] & 0xFFFF0000u)};
+          __builtin_amdgcn_raw_buffer_store_b64(codes, rq, in ? static_cast<uint32_t>(row * ldq + c / 2 + 8 * grp) : 0x80000000u, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(byte), rs,
+                                               grp == 0 ? row * kMxTileBlocks + mx_scale_pos(b & 15) : 0x80000000u, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);  // one fragment at a time: the next tile's operands are in registers already
+        }
+      }
+    } else if constexpr (kSplit) {
       float* part = g.part + kpart * g.M * g.N;
 #pragma unroll
       for (int i = 0; i < kFM; ++i) {
@@ -336,8 +424,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
           }
       }
     } else if (g.store == 8) {
-      // lanes l and l + 32 swap halves: 8 adjacent columns of row 32 i + r32
-      // each, one 16-byte store; rows past M lie past the view
+      // Lanes l and l + 32 swap halves: 8 adjacent columns of row 32 i + r32
+      // each; then 16-lane groups swap between two such vectors: 16 rows of 64
+      // contiguous bytes per 16-byte store.  Rows past M lie past the view.
       const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
           scalar_ptr(g.out + cur.m0 * g.N), 0, static_cast<int>(cur.rows_m * g.N * 2), kBufferFlags);
 #pragma unroll
@@ -358,15 +447,30 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
                                  static_cast<__bf16>(acc[i][j][2 * v + 1] + bias[2 * v + 1])};
             p[v] = __builtin_bit_cast(uint32_t, o);
           }
+          uint32_t o[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const auto x = __builtin_amdgcn_permlane32_swap(p[4 * h], p[4 * h + 2], false, false);
             const auto y = __builtin_amdgcn_permlane32_swap(p[4 * h + 1], p[4 * h + 3], false, false);
-            const int64_t n = nw + 32 * j + 16 * h + 8 * grp;
-            const uint32_t off = n < g.N ? static_cast<uint32_t>(((wm * kWaveM + 32 * i + r32) * g.N + n) * 2) : 0x80000000u;
-            typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-            __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, ro, off, 0, 0);
+            o[h][0] = x[0];
+            o[h][1] = y[0];
+            o[h][2] = x[1];
+            o[h][3] = y[1];
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const auto x = __builtin_amdgcn_permlane16_swap(o[0][k], o[1][k], false, false);
+            o[0][k] = x[0];
+            o[1][k] = x[1];
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // rows 16 h + l % 16, lane groups 0 .. 3 on 8-column chunks 0, 2, 1, 3
+            const int64_t n = nw + 32 * j + 8 * ((lane >> 4 & 1) * 2 + grp);
+            const uint32_t off = n < g.N ? static_cast<uint32_t>(((wm * kWaveM + 32 * i + 16 * h + (lane & 15)) * g.N + n) * 2) : 0x80000000u;
+            typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4{o[h][0], o[h][1], o[h][2], o[h][3]}, ro, off, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     } else {

@@ -94,6 +94,9 @@ SIGNATURES = {
     "mw8_set_mxfp4_tuning": (None, [_I32, _I32]),
     "mw8_mxfp4_tuning_count": (_I32, []),
     "mw8_linear_bf16_mxfp4": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "mw8_gemm_act_mxfp4": (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P]),
+    "mw8_gemm_act_mxfp4_supported": (_I32, [_I64, _I64, _I64]),
+    "mw8_gemm_act_mxfp4_preferred": (_I32, [_I64, _I64, _I64]),
     "mw8_linear_bf16_mxfp4_supported": (_I32, [_I64, _I64, _I64]),
     "mw8_rotary_qk": (
         ctypes.c_int,

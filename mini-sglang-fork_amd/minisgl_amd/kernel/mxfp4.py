@@ -197,6 +197,30 @@ def _gemm(q, s_a, w, s_w, bias, y, M: int, N: int) -> None:
                                   M, N, K, _ptr(ws), need, _stream(q)))
 
 
+def gemm_act_mxfp4(
+    q: torch.Tensor, s_a: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, activation: str = "silu"
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scale) of act(gate) * up [M, I] for the quantized A [M, K] and
+    gate_up weight [2I, K]: one launch, the bits of ``gemm_mxfp4`` followed by
+    ``act_and_mul_quant_mxfp4``.  I % 32 == 0."""
+    _one_gpu(q, s_a, w, s_w)
+    _need(activation in _ACT, f"unsupported activation {activation}")
+    M, N = _check_operand("A", q, s_a, None), _check_operand("W", w, s_w, None)
+    _need(q.shape[1] == w.shape[1], "A/W K mismatch")
+    _need(N > 0 and N % 64 == 0, "W: 2I rows, I a multiple of 32")
+    codes, scale = _empty(M, N // 2, q)
+    if M > 0:
+        with _device_of(q):
+            check(load().mw8_gemm_act_mxfp4(_ptr(q), _ptr(s_a), _ptr(w), _ptr(s_w), _ACT[activation], _ptr(codes),
+                                            _ptr(scale), M, N // 2, q.shape[1] * 2, _stream(q)))
+    return codes, scale
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [M, K] with contiguous, separate rows (x itself, or a copy)."""
+    return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
 def linear_mxfp4(
     x: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, bias: Optional[torch.Tensor] = None
 ) -> torch.Tensor:
@@ -207,8 +231,7 @@ def linear_mxfp4(
     _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "linear_mxfp4: x must be bf16 [..., K]")
     N = _check_operand("W", w, s_w, x.shape[-1])
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
-        x2 = x2.contiguous()
+    x2 = _rows(x2)
     M, K = x2.shape
     _check_bias_out(bias, None, M, N)
     if 0 < M <= 16 and x2.data_ptr() % 16 == 0 and (M == 1 or x2.stride(0) % 8 == 0):
@@ -238,14 +261,29 @@ def gated_mlp_mxfp4(
     """down(act(gate(x)) * up(x)) on quantized weights gate_up [2I, H] (gate
     rows first) and down [H', I]: bf16 x [..., H] -> bf16 [..., H'].  gate,
     up and their product are rounded to bf16 before the product is
-    quantized for down."""
+    quantized for down.  Large batches run gate_up, activation and
+    quantizer as one launch (``gemm_act_mxfp4``)."""
     _one_gpu(x, w_gate_up, s_gate_up, w_down, s_down)
     _need(activation in _ACT, f"unsupported activation {activation}")
     _need(w_gate_up.dim() == 2 and w_gate_up.shape[0] > 0 and w_gate_up.shape[0] % 2 == 0, "w_gate_up: 2I rows")
     inter = w_gate_up.shape[0] // 2
     N = _check_operand("down", w_down, s_down, inter)
-    gu = linear_mxfp4(x, w_gate_up, s_gate_up)
-    y = gemm_mxfp4(*act_and_mul_quant_mxfp4(gu.view(-1, 2 * inter), activation), w_down, s_down)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    M, K = x2.shape
+    if M == 0:
+        y = torch.empty((0, N), dtype=torch.bfloat16, device=x.device)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+    with _device_of(x):
+        fused = M > 16 and load().mw8_gemm_act_mxfp4_preferred(M, inter, K)
+    if fused:
+        _need(x.dtype == torch.bfloat16, "gated_mlp_mxfp4: x must be bf16 [..., H]")
+        _check_operand("gate_up", w_gate_up, s_gate_up, K)
+        codes, scale = gemm_act_mxfp4(*quant_mxfp4(_rows(x2)), w_gate_up, s_gate_up, activation)
+    else:
+        codes, scale = act_and_mul_quant_mxfp4(linear_mxfp4(x2, w_gate_up, s_gate_up), activation)
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    with _device_of(x):
+        _gemm(codes, scale, w_down, s_down, None, y, M, N)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
@@ -253,6 +291,7 @@ __all__ = [
     "act_and_mul_quant_mxfp4",
     "dequant_mxfp4",
     "gated_mlp_mxfp4",
+    "gemm_act_mxfp4",
     "gemm_mxfp4",
     "linear_mxfp4",
     "mxfp4_row_scales",

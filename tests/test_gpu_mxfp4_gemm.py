@@ -284,3 +284,38 @@ def test_workspace():
     y.zero_()
     check(lib.mw8_gemm_mxfp4_bf16(*args, None, 0, st))
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,I,K", [(1, 32, 32), (3, 96, 544), (100, 160, 1024), (257, 128, 480), (300, 768, 2048),
+                                   (700, 1504, 512), (2080, 544, 1024), (5000, 2048, 256)])
+def test_gemm_act_equals_its_parts(act, M, I, K):
+    """gate_up product, activation and quantizer in one launch: the codes and
+    scale bytes of the three on exact inputs (any fp32 order gives the same
+    sums), bytes past I included; a NaN reaches its row's blocks only."""
+    from minisgl_amd.kernel import act_and_mul_quant_mxfp4, gemm_act_mxfp4
+
+    announce(f"gemm_act_mxfp4 M={M} I={I} K={K} {act}")
+    a, _ = _operand(M, K, seed=M)
+    w, _ = _operand(2 * I, K, seed=I, low=118, high=119)
+    a[1][0, M // 2, 0] = 255
+    want = act_and_mul_quant_mxfp4(gemm_mxfp4(*a, *w), act)
+    got = gemm_act_mxfp4(*a, *w, act)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_gemm_act_refusals():
+    from minisgl_amd.kernel import gemm_act_mxfp4, load
+
+    a, _ = _operand(4, 512, seed=1)
+    for rows in (40, 66):
+        w, _ = _operand(rows, 512, seed=2)
+        with pytest.raises(ValueError):
+            gemm_act_mxfp4(*a, *w)
+    w, _ = _operand(64, 512, seed=2)
+    with pytest.raises(ValueError):
+        gemm_act_mxfp4(*a, *w, "relu")
+    assert gemm_act_mxfp4(a[0][:0], a[1][:, :0].contiguous(), *w)[0].shape == (0, 16)
+    lib = load()
+    assert lib.mw8_gemm_act_mxfp4_supported(1, 32, 1) and not lib.mw8_gemm_act_mxfp4_supported(1, 33, 32)
+    assert not lib.mw8_gemm_act_mxfp4_supported(1, 1 << 21, 1 << 11)
