@@ -264,33 +264,59 @@ def gated_mlp_mxfp4(
     quantized for down.  Large batches run gate_up, activation and
     quantizer as one launch (``gemm_act_mxfp4``)."""
     _one_gpu(x, w_gate_up, s_gate_up, w_down, s_down)
-    _need(activation in _ACT, f"unsupported activation {activation}")
-    _need(w_gate_up.dim() == 2 and w_gate_up.shape[0] > 0 and w_gate_up.shape[0] % 2 == 0, "w_gate_up: 2I rows")
-    inter = w_gate_up.shape[0] // 2
-    N = _check_operand("down", w_down, s_down, inter)
+    _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "gated_mlp_mxfp4: x must be bf16 [..., H]")
+    inter, N = _check_mlp(x.shape[-1], w_gate_up, s_gate_up, w_down, s_down, activation)
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    M, K = x2.shape
-    if M == 0:
-        y = torch.empty((0, N), dtype=torch.bfloat16, device=x.device)
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
-    with _device_of(x):
-        fused = M > 16 and load().mw8_gemm_act_mxfp4_preferred(M, inter, K)
-    if fused:
-        _need(x.dtype == torch.bfloat16, "gated_mlp_mxfp4: x must be bf16 [..., H]")
-        _check_operand("gate_up", w_gate_up, s_gate_up, K)
+    if _fused_act(x2.shape[0], inter, x2.shape[1], x2):
         codes, scale = gemm_act_mxfp4(*quant_mxfp4(_rows(x2)), w_gate_up, s_gate_up, activation)
     else:
         codes, scale = act_and_mul_quant_mxfp4(linear_mxfp4(x2, w_gate_up, s_gate_up), activation)
-    y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
-    with _device_of(x):
-        _gemm(codes, scale, w_down, s_down, None, y, M, N)
+    y = gemm_mxfp4(codes, scale, w_down, s_down)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
+def gated_mlp_quantized_mxfp4(
+    codes: torch.Tensor,
+    scale: torch.Tensor,
+    w_gate_up: torch.Tensor,
+    s_gate_up: torch.Tensor,
+    w_down: torch.Tensor,
+    s_down: torch.Tensor,
+    activation: str = "silu",
+) -> torch.Tensor:
+    """``gated_mlp_mxfp4`` of rows that are quantized already (codes, scale
+    of [M, H], as ``rmsnorm_quant_mxfp4`` gives them): bf16 [M, H']."""
+    _one_gpu(codes, scale, w_gate_up, s_gate_up, w_down, s_down)
+    M, K = _check_operand("x", codes, scale, None), codes.shape[1] * 2
+    inter, _ = _check_mlp(K, w_gate_up, s_gate_up, w_down, s_down, activation)
+    if _fused_act(M, inter, K, codes):
+        codes, scale = gemm_act_mxfp4(codes, scale, w_gate_up, s_gate_up, activation)
+    else:
+        codes, scale = act_and_mul_quant_mxfp4(gemm_mxfp4(codes, scale, w_gate_up, s_gate_up), activation)
+    return gemm_mxfp4(codes, scale, w_down, s_down)
+
+
+def _check_mlp(K: int, w_gate_up, s_gate_up, w_down, s_down, activation: str) -> Tuple[int, int]:
+    """(I, output size) of a gated MLP on rows of K."""
+    _need(activation in _ACT, f"unsupported activation {activation}")
+    rows = _check_operand("gate_up", w_gate_up, s_gate_up, K)
+    _need(rows > 0 and rows % 2 == 0, "gate_up: 2I rows")
+    return rows // 2, _check_operand("down", w_down, s_down, rows // 2)
+
+
+def _fused_act(M: int, inter: int, K: int, like: torch.Tensor) -> bool:
+    """Whether gate_up, activation and quantizer run as one launch."""
+    if M <= 16:
+        return False
+    with _device_of(like):
+        return bool(load().mw8_gemm_act_mxfp4_preferred(M, inter, K))
 
 
 __all__ = [
     "act_and_mul_quant_mxfp4",
     "dequant_mxfp4",
     "gated_mlp_mxfp4",
+    "gated_mlp_quantized_mxfp4",
     "gemm_act_mxfp4",
     "gemm_mxfp4",
     "linear_mxfp4",

@@ -123,3 +123,29 @@ def test_python_refuses_cpu_tensors():
         mxfp4_tile_scales(torch.zeros(2, 3))
     with pytest.raises(ValueError):
         mxfp4_row_scales(s, 1024)
+
+
+def test_layers_state_and_refusals():
+    from minisgl_amd.layers import GatedMLPMXFP4, LinearMXFP4, RMSNormQuantMXFP4
+
+    layer = LinearMXFP4(1000, [64, 32], has_bias=True)
+    assert layer.weight.shape == (96, 512) and layer.weight_scale.shape == (2, 96, 16) and layer.bias.shape == (96,)
+    assert set(layer.state_dict()) == {"weight", "weight_scale", "bias"}
+    codes = torch.zeros(96, 512, dtype=torch.uint8)
+    rows = torch.randint(0, 255, (96, 32), dtype=torch.uint8)
+    layer.load_mxfp4_weight(codes, rows, torch.ones(96))
+    assert torch.equal(mxfp4_row_scales(layer.weight_scale, 1000), rows) and layer.bias.dtype == torch.bfloat16
+    for bad in (
+        lambda: layer.load_mxfp4_weight(codes[:, :500], rows),
+        lambda: layer.load_mxfp4_weight(codes, rows[:, :31]),
+        lambda: layer.load_mxfp4_weight(codes.int(), rows),
+        lambda: layer.load_mxfp4_weight(codes, rows, torch.ones(95)),
+        lambda: layer.load_float_weight(torch.zeros(96, 999)),
+        lambda: layer.forward(torch.zeros(2, 1000, dtype=torch.bfloat16)),
+        lambda: GatedMLPMXFP4(64, 64, "relu"),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+    mlp = GatedMLPMXFP4(512, 256)
+    assert mlp.gate_up_proj.output_size == 512 and mlp.down_proj.weight.shape == (512, 128)
+    assert RMSNormQuantMXFP4(64, 1e-6).state_dict()["weight"].shape == (64,)
