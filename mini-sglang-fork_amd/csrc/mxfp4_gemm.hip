@@ -35,20 +35,20 @@ constexpr int kLdsBytes = 163840;
 
 // ------------------------------------------------------------------- rings
 // Tilings and what the time model knows of them (MI355X, fitted to graph-timed
-// runs of 70 random shapes from 17 to 8192 rows): us = start + (rounds - 1)
+// runs of 130 random shapes from 17 to 8192 rows): us = start + (rounds - 1)
 // round + max(latency stages rounds, rate stages tiles per CU), at least
-// start + the operands at bw TB/s.  The pick is 2% off the fastest
-// configuration on average, 35% at most (230 x 34816 x 5120).
+// start + the operands and the output at bw TB/s.  On those shapes the pick is
+// 0.5% off the fastest configuration on average and 13% at most (78 x 51200 x 5120).
 struct MxRingCfg {
   int bm, bn, per_cu;
   float start, round, latency, rate, bw;
 };
 constexpr MxRingCfg kMxRings[] = {
-    {256, 256, 1, 4.51f, 14.31f, 1.446f, 0.337f, 3.05f},  // 0: a block per CU walks its tiles
-    {256, 192, 1, 3.97f, 9.85f, 1.178f, 0.282f, 2.60f},   // 1: likewise
-    {128, 128, 2, 3.15f, 4.18f, 0.774f, 0.554f, 3.94f},   // 2: likewise, two blocks per CU
-    {128, 128, 1, 4.03f, 4.89f, 0.544f, 0.474f, 4.13f},   // 3: four stages in flight
-    {64, 64, 2, 3.39f, 2.13f, 0.277f, 0.229f, 3.73f},     // 4: likewise; the one that splits K
+    {256, 256, 1, 5.19f, 6.50f, 1.559f, 1.608f, 3.40f},  // 0: a block per CU walks its tiles
+    {256, 192, 1, 4.44f, 4.27f, 1.308f, 0.914f, 3.52f},  // 1: likewise
+    {128, 128, 2, 3.79f, 2.20f, 0.695f, 0.588f, 3.64f},  // 2: likewise, two blocks per CU
+    {128, 128, 1, 4.23f, 3.95f, 0.573f, 0.397f, 4.32f},  // 3: four stages in flight
+    {64, 64, 2, 3.38f, 1.55f, 0.271f, 0.243f, 5.11f},    // 4: likewise; the one that splits K
 };
 constexpr int kNumMxRings = sizeof(kMxRings) / sizeof(kMxRings[0]);
 constexpr int kMxSplitCfg = 4, kMxMaxSplit = 16, kMxDecodeRows = 16;
@@ -69,7 +69,7 @@ double mx_ring_us(int c, int64_t M, int64_t N, int64_t K, int split) {
   const double bytes = static_cast<double>(N) * K * (17.0 / 32) + 2.0 * M * N;
   us = std::max(us, r.start + bytes / (r.bw * 1e6));
   // the sums' way through memory and the second launch
-  if (split > 1) us += 2.3 + 8.0 * split * M * N / 4.4e6;
+  if (split > 1) us += 2.1 + 8.0 * split * M * N / 3.9e6;
   return us;
 }
 
@@ -109,6 +109,11 @@ int launch_ring(MxArgs g, hipStream_t st) {
   const int64_t all = tm * tn * g.split, blocks = NS == 2 ? std::min(all, slots) : all;
   MW8_REQUIRE(blocks * kThreads < (1ll << 32), kErrShape, "gemm_mxfp4: M=%lld x N=%lld too large", (long long)g.M,
               (long long)g.N);
+  // From eight rounds and K = 4096 on the last group's late start costs less
+  // than the stores' bursts (MI355X, us, together -> staggered: 8192 x 34816 x
+  // 5120 748 -> 716, 4096 rows 391 -> 369, 8192 x 51200 x 5120 1139 -> 1125; but 2080
+  // x 51200 x 5120, 7 rounds, 310 -> 318, and 8192 x 16384 x 2048 159 -> 171).
+  if (BM == 256 && BN == 256 && tm * tn >= 8 * blocks && g.tiles >= 8) g.stagger = g.tiles * 4 / 5;
   if (const int rc = mx_lds_limit<kern>(R::kLds)) return rc;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), R::kLds, st, g);
   return check_launch("gemm_mxfp4");
@@ -174,7 +179,7 @@ MxArgs mx_args(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint
   // (16-byte stores go through a 32-bit view of a tile's output rows)
   const int store = N % 8 == 0 && aligned_to(y, 16) && N < (1ll << 22) ? 8 : N % 4 == 0 && aligned_to(y, 8) ? 4 : 1;
   return {A, sa, W, sw, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), M, N,
-          static_cast<int>(mx_blocks(K)), static_cast<int>(mx_tiles(K)), store, {}, nullptr, 1, nullptr, nullptr};
+          static_cast<int>(mx_blocks(K)), static_cast<int>(mx_tiles(K)), store, {}, nullptr, 1, 0, nullptr, nullptr};
 }
 
 }  // namespace

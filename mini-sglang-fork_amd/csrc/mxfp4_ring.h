@@ -61,6 +61,9 @@ struct MxArgs {
   // b % count, p = b / count, and writes fp32 sums to part[p][M][N]
   float* part;
   int split;
+  // long walks: blocks start in four groups, a quarter of a tile apart (units
+  // of 2048 clocks)
+  int stagger;
   // kAct kernels: W [2 I, K] holds gate rows, then up rows (N = 2 I); the output
   // is the quantized activation [M, I]
   uint8_t* q;
@@ -322,6 +325,13 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
   using I1 = std::integral_constant<int, 1>;
   using Stores = std::integral_constant<int, kStores>;
 
+  // The blocks of a walk finish their tiles together, and 256 CUs that store
+  // 128 KB each at once wait for memory (a wave's stores retire before its
+  // later loads).  Apart from each other by a quarter of a tile, the stores
+  // of one group run under the products of the others.
+  if constexpr (kWalk && kAct < 0) {
+    for (int i = static_cast<int>(blockIdx.x * 4 / gridDim.x) * g.stagger; i > 0; --i) __builtin_amdgcn_s_sleep(32);
+  }
   uint32_t t = blockIdx.x - kpart * count;
   Tile cur = tile_at(t);
   Tile none = cur;
