@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256) void rotary_generic_kernel(RotArgs a) {
 // LPH lanes own a head.  A block takes one token and walks its heads, so a
 // lane loads its cosines, sines and norm weights once.  Every element is read
 // and written once; the bound is HBM (MI355X: 8000 tokens x 40 heads of 128,
-// fp16, 64 rotated, @T1@).
+// fp16, 64 rotated, into other tensors 32 us, 5.2 TB/s; in place 27 us; one
+// token of 72 heads with norms 3.8 us).
 template <class E, bool kInter>
 __global__ __launch_bounds__(1024) void rotary_rows_kernel(RotArgs a, int lph) {
   constexpr int V = 16 / sizeof(E);
@@ -187,7 +188,7 @@ __device__ __forceinline__ void angle_of(double p, double f, double& s, double& 
 // fp64.  A thread fills kTableRows positions from two sines: the next angle
 // comes by cos(x + y) = cos x cos y - sin x sin y (the error grows by a few
 // 2^-53 a step), 4 multiplications in place of a sine.  Bound: the stores
-// (MI355X: 131072 x 128 @T2@).
+// (MI355X: 131072 x 128 in 12.9 us, 5.2 TB/s; a sine per element took 33 us).
 constexpr int kTableRows = 8;
 __global__ __launch_bounds__(256) void rotary_table_kernel(const double* __restrict__ freq, uint32_t half, int64_t P,
                                                            double scale, float* __restrict__ table) {
