@@ -76,6 +76,7 @@ def rotary_qk(
           "q_out and k_out: as q and k")
     if T == 0 or hq + hk == 0:
         return q_out, k_out
+    _need(hq == 0 or hk == 0 or q_out.data_ptr() != k_out.data_ptr(), "q_out and k_out must not overlap")
     qs, ks = _strides("q", q), _strides("k", k)
     qos = qs if q_out is q else _strides("q_out", q_out)
     kos = ks if k_out is k else _strides("k_out", k_out)

@@ -199,6 +199,7 @@ def test_rotary_refusals():
         lambda: rotary_qk(q, k, pos, table, q_weight=w.float()),
         lambda: rotary_qk(q, k, pos, table, k_weight=w[:32]),
         lambda: rotary_qk(q, k, pos, table, q_out=q[:, :1]),
+        lambda: rotary_qk(q, q, pos, table),
         lambda: rotary_qk(q.transpose(1, 2), k, pos, table),
         lambda: rotary_qk(q[:, :1].expand(4, 2, 64), k, pos, table),
         lambda: rotary_cos_sin(torch.ones(4, device=DEV), 8),
