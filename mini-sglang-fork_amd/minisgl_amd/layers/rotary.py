@@ -140,8 +140,8 @@ class RotaryEmbedding(StateLessOP):
             raise ValueError("q_norm and k_norm must have the same eps")
         norm = q_norm if q_norm is not None else k_norm
         rotary_qk(
-            query if query.dim() == 3 else query.view(query.shape[0], -1, self.head_size),
-            key if key.dim() == 3 else key.view(key.shape[0], -1, self.head_size),
+            self._heads(query),
+            self._heads(key),
             positions,
             self.prepare(query.device),
             interleaved=self.interleaved,
@@ -150,6 +150,15 @@ class RotaryEmbedding(StateLessOP):
             eps=0.0 if norm is None else norm.eps,
         )
         return query, key
+
+    def _heads(self, x: torch.Tensor) -> torch.Tensor:
+        """x [T, heads * D] or [T, heads, D] as [T, heads, D]."""
+        D = self.head_size
+        if x.dim() == 3 and x.shape[2] == D:
+            return x
+        if x.dim() == 2 and x.shape[1] % D == 0:
+            return x.view(x.shape[0], x.shape[1] // D, D)
+        raise ValueError(f"query and key: [T, heads * {D}] or [T, heads, {D}], got {tuple(x.shape)}")
 
 
 __all__ = ["RotaryEmbedding", "rotary_frequencies"]

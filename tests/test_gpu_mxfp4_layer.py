@@ -170,6 +170,9 @@ def test_rotary_layer_refuses_its_first_use_in_a_capture():
     rope.forward(p, q, k)
     with pytest.raises(ValueError, match="eps"):
         rope.forward(p, q, k, RMSNorm(64, 1e-5), RMSNorm(64, 1e-6))
+    with pytest.raises(ValueError, match="heads"):
+        rope.forward(p, q[:, :100], k)
+    rope.forward(p[:0], q[:0], k[:0])
 
 
 def test_norm_layer_with_strided_residual():
