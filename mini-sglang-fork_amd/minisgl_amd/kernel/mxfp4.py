@@ -234,12 +234,14 @@ def linear_mxfp4(
     x2 = _rows(x2)
     M, K = x2.shape
     _check_bias_out(bias, None, M, N)
-    if 0 < M <= 16 and x2.data_ptr() % 16 == 0 and (M == 1 or x2.stride(0) % 8 == 0):
+    ldx = K if M <= 1 else x2.stride(0)
+    # (the one launch reads x through a 32-bit view: rows less than 2^26 elements apart)
+    if 0 < M <= 16 and x2.data_ptr() % 16 == 0 and (M == 1 or (ldx % 8 == 0 and ldx < 1 << 26)):
         lib = load()
         with _device_of(x):
             if lib.mw8_linear_bf16_mxfp4_supported(M, N, K):
                 y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
-                check(lib.mw8_linear_bf16_mxfp4(x2.data_ptr(), max(x2.stride(0), K), w.data_ptr(), s_w.data_ptr(), _ptr(bias),
+                check(lib.mw8_linear_bf16_mxfp4(x2.data_ptr(), ldx, w.data_ptr(), s_w.data_ptr(), _ptr(bias),
                                                 y.data_ptr(), M, N, K, _stream(x)))
                 return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
     y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)

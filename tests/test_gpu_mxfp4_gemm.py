@@ -122,6 +122,19 @@ def test_linear_layouts(M):
     assert torch.isnan(y[0]).all() and torch.equal(y[1:], want[1:])
 
 
+@pytest.mark.parametrize("M", [1, 2])
+def test_linear_of_rows_far_apart(M):
+    """Last tokens of long sequences: rows 2^26 elements and more apart."""
+    K, far = 512, (1 << 26) + 8
+    announce(f"linear_mxfp4 M={M} rows {far} apart")
+    w, _ = _operand(64, K, seed=1)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).bfloat16().to(DEV)
+    store = torch.empty((M - 1) * far + K, dtype=torch.bfloat16, device=DEV)
+    view = store.as_strided((M, K), (far, 1))
+    view.copy_(x)
+    assert torch.equal(linear_mxfp4(view, *w), linear_mxfp4(x, *w))
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("M,H,I", [(1, 512, 768), (5, 1000, 500), (16, 2048, 768), (70, 512, 640), (300, 1024, 1056),
                                    (1100, 512, 384)])
