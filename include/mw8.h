@@ -482,7 +482,7 @@ int32_t mw8_linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K);
  * W [2I, K] (gate rows, then up rows) -> q, s of bf16(act(gate) * up) [M, I],
  * gate and up rounded to bf16 first: bit-identical to mw8_gemm_mxfp4_bf16 +
  * mw8_act_and_mul_quant_mxfp4_bf16.  q 8-byte aligned.  _supported (host
- * only): I % 32 == 0, the codes of W below 2 GiB; _preferred: whether it is
+ * only): I % 32 == 0, I < 2^24, the codes of W below 2 GiB; _preferred: whether it is
  * also the faster way (larger batches).
  */
 int mw8_gemm_act_mxfp4(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int32_t act, uint8_t* q,

@@ -222,9 +222,9 @@ int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const
 }
 
 // Whether gemm_act_mxfp4 takes (M, I, K): whole blocks of activation columns,
-// the weight within a 32-bit view.
+// the weight and 256 rows of codes within 32-bit views.
 int gemm_act_mxfp4_supported(int64_t M, int64_t I, int64_t K) {
-  return M > 0 && I > 0 && K > 0 && K <= (1ll << 20) && I % kMxBlock == 0 && I < (1ll << 30) &&
+  return M > 0 && I > 0 && K > 0 && K <= (1ll << 20) && I % kMxBlock == 0 && I < (1ll << 24) &&
          2 * I * mx_blocks(K) * 16 < (1ll << 31) && M < (1ll << 31);
 }
 

@@ -105,6 +105,15 @@ def test_c_refusals():
     assert lib.mw8_last_error()
 
 
+def test_fused_activation_limits():
+    """256 rows of output codes must fit a 32-bit view: I / 2 * 256 < 2^31."""
+    lib = load()
+    p = ctypes.c_void_p(4096)
+    assert lib.mw8_gemm_act_mxfp4_supported(256, (1 << 24) - 32, 32) == 1
+    assert lib.mw8_gemm_act_mxfp4_supported(256, 1 << 24, 32) == 0
+    assert lib.mw8_gemm_act_mxfp4(p, p, p, p, 0, p, p, 256, 1 << 24, 32, None) == 2
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     w, s = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(1, 8, 16, dtype=torch.uint8)
