@@ -430,7 +430,7 @@ int mw8_moe_sum_reduce_bf16(const void* in, int64_t M, int32_t k, int64_t H, voi
  */
 
 /* x bf16 [M, K] (row stride ldx >= K elements, any K) -> q, s.  x 2-byte, q 4-byte aligned
- * (16-byte loads where x, K and ldx allow). */
+ * (16-byte loads where x, K and ldx allow); ceil(M / 4) ceil(K / 512) <= 2^26 - 4. */
 int mw8_quant_mxfp4_bf16(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* q, uint8_t* s,
                          mw8_stream_t stream);
 
@@ -442,7 +442,7 @@ int mw8_act_and_mul_quant_mxfp4_bf16(const void* x, int64_t R, int64_t two_d, in
 int mw8_rmsnorm_quant_mxfp4_bf16(const void* x, void* residual, const void* weight, float eps, int64_t M, int64_t H,
                                  uint8_t* q, uint8_t* s, void* y, mw8_stream_t stream);
 
-/* y bf16 [M, K]: the values that q, s stand for (NaN where a scale byte is 255). */
+/* y bf16 [M, K]: the values that q, s stand for (NaN where a scale byte is 255); M ceil(K / 512) <= 2^26 - 4. */
 int mw8_dequant_mxfp4_bf16(const uint8_t* q, const uint8_t* s, int64_t M, int64_t K, void* y, mw8_stream_t stream);
 
 /*

@@ -170,6 +170,8 @@ int launch_decode(const MxDecodeArgs& d, const MxDecodePlan& p, hipStream_t st) 
   const int lds = mx_decode_lds(p, d.g.M, d.K, kXQ);
   if (const int rc = mx_lds_limit<kern>(kLdsBytes)) return rc;
   const int64_t cus = device_cus(), blocks = cus * ((d.g.N + cus * 16 * RG - 1) / (cus * 16 * RG));
+  MW8_REQUIRE(blocks * 64 * p.waves < (1ll << 32), kErrShape, "gemm_mxfp4: N=%lld x K=%lld too large", (long long)d.g.N,
+              (long long)d.K);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * p.waves), lds, st, d);
   return check_launch("gemm_mxfp4");
 }

@@ -113,10 +113,11 @@ __global__ __launch_bounds__(kMxThreads) void dequant_mxfp4_kernel(const uint8_t
 
 inline bool aligned_to(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
-// blocks of kMxWaves waves over ceil(M / U) row groups x tiles; 0: too many
+// blocks of kMxWaves waves over ceil(M / U) row groups x tiles; 0: too many (a
+// launch holds fewer than 2^32 threads, one wave is 64 of them)
 unsigned mx_grid(int64_t M, int64_t K, int U) {
   const int64_t groups = (M + U - 1) / U, tiles = mx_tiles(K);
-  if (groups > ((1ll << 31) - 1) / tiles) return 0;
+  if (groups > ((1ll << 26) - kMxWaves) / tiles) return 0;
   return static_cast<unsigned>((groups * tiles + kMxWaves - 1) / kMxWaves);
 }
 

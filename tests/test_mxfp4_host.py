@@ -114,6 +114,18 @@ def test_fused_activation_limits():
     assert lib.mw8_gemm_act_mxfp4(p, p, p, p, 0, p, p, 256, 1 << 24, 32, None) == 2
 
 
+def test_launch_limits():
+    """A launch holds fewer than 2^32 threads: one wave per row (or four rows)
+    and 512 elements, four waves a block."""
+    lib = load()
+    p = ctypes.c_void_p(4096)
+    rows = 1 << 26
+    assert lib.mw8_dequant_mxfp4_bf16(p, p, rows, 32, p, None) == 2
+    assert lib.mw8_dequant_mxfp4_bf16(p, p, rows // 8, 4096, p, None) == 2
+    assert lib.mw8_quant_mxfp4_bf16(p, 4 * rows, 32, 32, p, p, None) == 2
+    assert lib.mw8_act_and_mul_quant_mxfp4_bf16(p, 4 * rows, 64, 0, p, p, None) == 2
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     w, s = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(1, 8, 16, dtype=torch.uint8)
