@@ -101,7 +101,7 @@ def rmsnorm_quant_mxfp4(
     """``rmsnorm_quant`` with the MXFP4 quantizer: bf16 x [M, H] -> (codes,
     scale[, bf16 y [M, H]]) of the normalized rows, bit-identical to
     ``quant_mxfp4`` of its y.  ``residual`` is added first and updated in
-    place; ``y`` may be ``x``.  H % 8 == 0, H <= 32768."""
+    place; ``y`` may be ``x``, not ``residual``.  H % 8 == 0, H <= 32768."""
     _one_gpu(x, weight, residual, y)
     _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(), "x: bf16 [M, H] contiguous")
     M, H = x.shape
@@ -115,6 +115,7 @@ def rmsnorm_quant_mxfp4(
         y = torch.empty((M, H), dtype=torch.bfloat16, device=x.device)
     if y is not None:
         _need(y.dtype == torch.bfloat16 and y.shape == (M, H) and y.is_contiguous(), "y: bf16 [M, H]")
+        _need(M == 0 or residual is None or y.data_ptr() != residual.data_ptr(), "y must not be residual")
     codes, scale = _empty(M, H, x)
     if M > 0:
         with _device_of(x):

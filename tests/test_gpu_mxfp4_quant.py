@@ -179,6 +179,14 @@ def test_rmsnorm_quant_in_place_and_nan():
     assert (rows[1] == 255).all() and (rows[2] == 0).all() and (rows[0] < 255).all()
 
 
+def test_rmsnorm_quant_refuses_y_on_residual():
+    """Both are written: the sum and the normalized row."""
+    x, r = (torch.ones(4, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    with pytest.raises(ValueError, match="residual"):
+        rmsnorm_quant_mxfp4(x, x[0], 1e-6, residual=r, y=r)
+    assert (r == 1).all()
+
+
 def test_empty_and_refusals():
     x = torch.zeros(0, 64, dtype=torch.bfloat16, device=DEV)
     codes, scale = quant_mxfp4(x)
