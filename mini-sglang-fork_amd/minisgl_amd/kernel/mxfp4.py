@@ -166,6 +166,9 @@ def _check_bias_out(bias, out, M: int, N: int) -> None:
         _need(bias.dtype == torch.bfloat16 and bias.shape == (N,) and bias.is_contiguous(), "bias: bf16 [N]")
     if out is not None:
         _need(out.dtype == torch.bfloat16 and out.shape == (M, N) and out.is_contiguous(), "out: bf16 [M, N]")
+        if bias is not None:  # (blocks read it while others write)
+            b, o = bias.data_ptr(), out.data_ptr()
+            _need(b + 2 * N <= o or o + 2 * M * N <= b, "out must not overlap bias")
 
 
 def gemm_mxfp4(

@@ -195,6 +195,16 @@ def test_gemm_refusals():
             call()
 
 
+def test_gemm_refuses_out_on_bias():
+    a, _ = _operand(4, 512, seed=1)
+    w, _ = _operand(40, 512, seed=2)
+    out = torch.zeros(5, 40, dtype=torch.bfloat16, device=DEV)
+    for bias in (out[0], out[3], out.view(-1)[150:190]):
+        with pytest.raises(ValueError, match="overlap"):
+            gemm_mxfp4(*a, *w, bias=bias, out=out[:4])
+    gemm_mxfp4(*a, *w, bias=out[4], out=out[:4])
+
+
 @pytest.mark.parametrize("M", [1, 16, 64, 200, 1100])
 def test_streams_and_graph(M):
     """Eager on the current stream, on a side stream, and captured and replayed
