@@ -250,7 +250,8 @@ int rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int hq, const void* k, 
               void* q_out, int64_t qo_ld, int64_t qo_hd, void* k_out, int64_t ko_ld, int64_t ko_hd, int dtype, int D,
               int R, int interleaved, const void* pos, int pos64, const float* table, int64_t P, const void* qw,
               const void* kw, float eps, int64_t T, hipStream_t st) {
-  MW8_REQUIRE(T >= 0 && hq >= 0 && hk >= 0 && hq + hk > 0, kErrShape, "rotary_qk: bad sizes T=%lld heads=%d+%d",
+  const int64_t heads = static_cast<int64_t>(hq) + hk;
+  MW8_REQUIRE(T >= 0 && hq >= 0 && hk >= 0 && heads > 0, kErrShape, "rotary_qk: bad sizes T=%lld heads=%d+%d",
               (long long)T, hq, hk);
   MW8_REQUIRE(D > 0 && D <= 8192 && R > 0 && R <= D && R % 2 == 0, kErrShape,
               "rotary_qk: need an even rotary size in (0, head size <= 8192] (D=%d R=%d)", D, R);
@@ -260,10 +261,11 @@ int rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int hq, const void* k, 
   MW8_REQUIRE(eps >= 0.0f, kErrArg, "rotary_qk: eps must be >= 0");
   if (T == 0) return kOk;
   // (a launch holds fewer than 2^32 threads, here at most 64 per row or 256 per token)
-  MW8_REQUIRE(T < (1ll << 24) && T < (1ll << 26) / (hq + hk), kErrShape, "rotary_qk: too many rows");
+  MW8_REQUIRE(T < (1ll << 24) && T < (1ll << 26) / heads, kErrShape, "rotary_qk: too many rows");
   const unsigned size = dtype == 2 ? 4 : 2;
   auto al = [](const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; };
-  MW8_REQUIRE(al(q, size) && al(k, size) && al(q_out, size) && al(k_out, size) && al(table, 4) && al(pos, pos64 ? 8 : 4),
+  MW8_REQUIRE(al(q, size) && al(k, size) && al(q_out, size) && al(k_out, size) && al(table, 4) && al(pos, pos64 ? 8 : 4) &&
+                  al(qw, size) && al(kw, size),
               kErrAlign, "rotary_qk: tensors must be aligned to their elements");
   const RotArgs a{q, k, q_out, k_out, q_ld, q_hd, k_ld, k_hd, qo_ld, qo_hd, ko_ld, ko_hd, pos, table,
                   qw, kw, eps, T, P, hq, hk, D, R, pos64};

@@ -74,9 +74,12 @@ def rotary_qk(
     k_out = k if k_out is None else k_out
     _need(q_out.dtype == q.dtype and q_out.shape == q.shape and k_out.dtype == q.dtype and k_out.shape == k.shape,
           "q_out and k_out: as q and k")
+    _need(D <= 8192 and hq + hk < 1 << 26, "q and k: heads of at most 8192 elements, fewer than 2^26 heads")
     if T == 0 or hq + hk == 0:
         return q_out, k_out
-    _need(hq == 0 or hk == 0 or q_out.data_ptr() != k_out.data_ptr(), "q_out and k_out must not overlap")
+    if hq and hk:
+        _need(q_out.data_ptr() != k_out.data_ptr(), "q_out and k_out must not overlap")
+        _need(q_out.data_ptr() != k.data_ptr() and k_out.data_ptr() != q.data_ptr(), "q_out and k, k_out and q must not overlap")
     qs, ks = _strides("q", q), _strides("k", k)
     qos = qs if q_out is q else _strides("q_out", q_out)
     kos = ks if k_out is k else _strides("k_out", k_out)
@@ -92,8 +95,8 @@ def rotary_cos_sin(inv_freq: torch.Tensor, positions: int, scale: float = 1.0) -
     """The table of ``rotary_qk``: fp32 [positions, 2 * pairs], cos and sin of
     p * inv_freq[i] (inv_freq fp64 [pairs], the angle in fp64) times ``scale``."""
     _on_gpu(inv_freq)
-    _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.numel() > 0,
-          "inv_freq: fp64 [pairs]")
+    _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and 0 < inv_freq.numel() <= 4096,
+          "inv_freq: fp64 [pairs], at most 4096")
     _need(positions >= 0, "positions must be >= 0")
     half = inv_freq.numel()
     table = torch.empty((positions, 2 * half), dtype=torch.float32, device=inv_freq.device)

@@ -208,3 +208,22 @@ def test_rotary_refusals():
     ):
         with pytest.raises(ValueError):
             call()
+
+
+def test_rotary_refuses_crossed_outputs_and_sizes_past_the_entry():
+    """An output on the other input; a head, head count or frequency list
+    that a 32-bit argument cannot hold (views of a little memory)."""
+    q, k = (torch.zeros(4, h, 64, dtype=torch.bfloat16, device=DEV) for h in (2, 2))
+    pos, table = torch.arange(4, device=DEV), torch.ones(8, 64, device=DEV)
+    out = torch.zeros_like(q)
+    one = torch.zeros(1, dtype=torch.bfloat16, device=DEV)
+    for call in (
+        lambda: rotary_qk(q, k, pos, table, q_out=k, k_out=out),
+        lambda: rotary_qk(q, k, pos, table, q_out=out, k_out=q),
+        lambda: rotary_qk(one.expand(1, 1, 2**32 + 64), one.expand(1, 1, 2**32 + 64), pos[:1], table),
+        lambda: rotary_qk(one.expand(1, 2**32 + 1, 64), one.expand(1, 1, 64), pos[:1], table),
+        lambda: rotary_cos_sin(torch.ones(4097, dtype=torch.float64, device=DEV), 8),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    assert not out.any()

@@ -31,6 +31,19 @@ def test_c_refusals():
     assert lib.mw8_rotary_cos_sin(p, 4, 0, 1.0, p, None) == 0
 
 
+def test_c_refuses_many_heads_and_odd_weights():
+    lib = load()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4097)
+
+    def call(hq, hk, qw, kw):
+        return lib.mw8_rotary_qk(p, 128, 64, hq, p, 64, 64, hk, p, 128, 64, p, 64, 64, 0, 64, 64, 0, p, 1, p, 8, qw, kw, 1e-6, 4,
+                                 None)
+
+    for hq, hk in ((2**31 - 1, 1), (1, 2**31 - 1), (2**31 - 1, 2**31 - 1)):
+        assert call(hq, hk, None, None) == 2
+    assert call(2, 1, odd, None) == 3 and call(2, 1, None, odd) == 3
+
+
 def test_python_refuses_cpu_tensors():
     q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
