@@ -30,12 +30,14 @@ def rotary_frequencies(
       factor, those shorter than L0 / high_freq_factor kept, a linear blend
       in L0 / wavelength between;
     * ``yarn``: frequencies that turn more than beta_fast times over L0 are
-      kept, fewer than beta_slow divided by factor, a ramp between; cos and
-      sin times attention_factor (0.1 ln(factor) + 1, or the ratio of the
+      kept, fewer than beta_slow divided by factor, a ramp between (its ends
+      on whole indices unless ``truncate`` is false); cos and sin times attention_factor (0.1 ln(factor) + 1, or the ratio of the
       mscale terms where both are given).
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if not base > 1:
+        raise ValueError(f"base must be above 1, got {base}")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     scaling = scaling or {}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
@@ -72,8 +74,10 @@ def rotary_frequencies(
     def dim_of(turns: float) -> float:  # the (real) index whose frequency turns so often over the original context
         return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low = max(math.floor(dim_of(float(scaling.get("beta_fast") or 32))), 0)
-    high = min(math.ceil(dim_of(float(scaling.get("beta_slow") or 1))), rotary_dim - 1)
+    low, high = dim_of(float(scaling.get("beta_fast") or 32)), dim_of(float(scaling.get("beta_slow") or 1))
+    if scaling.get("truncate", True):
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, rotary_dim - 1)
     ramp = ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
     f = f / factor * ramp + f * (1 - ramp)
 
@@ -113,6 +117,8 @@ class RotaryEmbedding(StateLessOP):
     def prepare(self, device: torch.device) -> torch.Tensor:
         """The table on ``device``, built if it is not there yet."""
         dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError("the W8A8 HIP path needs GPU tensors (no CPU fallback)")
         index = torch.cuda.current_device() if dev.index is None else dev.index
         table = self._tables.get(index)
         if table is None:

@@ -79,3 +79,27 @@ def test_refusals(call):
 
 def test_layer_has_no_state():
     assert RotaryEmbedding(64, 64, 8, 1e4).state_dict() == {}
+
+
+def test_yarn_without_truncation():
+    """The ramp between the real-valued indices whose waves turn beta_fast
+    and beta_slow times over the original context."""
+    d, base, original, factor = 64, 1.5e5, 4096, 32.0
+    f, _ = rotary_frequencies(d, base, {"rope_type": "yarn", "factor": factor, "beta_fast": 32.0, "beta_slow": 1.0,
+                                        "original_max_position_embeddings": original, "truncate": False})
+    low, high = (d * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base)) for turns in (32.0, 1.0))
+    for i, got in enumerate(f.tolist()):
+        plain = base ** (-2 * i / d)
+        t = min(max((i - low) / (high - low), 0.0), 1.0)
+        assert got == pytest.approx(plain * (1 - t) + plain / factor * t, rel=1e-12)
+
+
+@pytest.mark.parametrize("base", [1.0, 0.0, -10000.0, float("nan")])
+def test_base_refused(base):
+    with pytest.raises(ValueError, match="base"):
+        rotary_frequencies(8, base)
+
+
+def test_prepare_refuses_the_cpu():
+    with pytest.raises(ValueError, match="GPU"):
+        RotaryEmbedding(64, 64, 8, 1e4).prepare(torch.device("cpu"))
