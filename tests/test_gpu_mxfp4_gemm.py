@@ -342,3 +342,54 @@ def test_gemm_act_refusals():
     lib = load()
     assert lib.mw8_gemm_act_mxfp4_supported(1, 32, 1) and not lib.mw8_gemm_act_mxfp4_supported(1, 33, 32)
     assert not lib.mw8_gemm_act_mxfp4_supported(1, 1 << 21, 1 << 11)
+
+
+def test_two_streams_at_once():
+    """Split products (fp32 sums in a workspace per call) queued on two streams
+    without a wait between them: the bits of one after the other."""
+    announce("split products on two streams")
+    w, _ = _operand(1024, 17408, seed=1, low=118, high=121)
+    a = [_operand(64, 17408, seed=2 + i, low=118, high=121)[0] for i in range(2)]
+    want = [gemm_mxfp4(*x, *w) for x in a]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(gemm_mxfp4(*a[i], *w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_other_threads_tuning_is_its_own():
+    """A tiling override holds on its thread only."""
+    import threading
+
+    from minisgl_amd.kernel import load
+
+    lib = load()
+    sizes = []
+
+    def other():
+        lib.mw8_set_mxfp4_tuning(0, 0)
+        sizes.append(lib.mw8_linear_bf16_mxfp4_supported(1, 512, 512))
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    thread.join()
+    sizes.append(lib.mw8_linear_bf16_mxfp4_supported(1, 512, 512))
+    assert sizes == [0, 1]
+
+
+@pytest.mark.parametrize("M", [1, 16, 17, 64, 333])
+def test_gemm_rows_behind_the_last(M):
+    """An out that is the head of a larger buffer: the rows behind it stay."""
+    announce(f"gemm_mxfp4 rows behind M={M}")
+    for N in (520, 517):
+        a, _ = _operand(M, 1024, seed=M)
+        w, _ = _operand(N, 1024, seed=N)
+        buf = torch.full((M + 300, N), 3.0, dtype=torch.bfloat16, device=DEV)
+        y = gemm_mxfp4(*a, *w, out=buf[:M])
+        assert torch.equal(y, gemm_mxfp4(*a, *w)) and (buf[M:] == 3).all()

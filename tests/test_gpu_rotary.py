@@ -227,3 +227,38 @@ def test_rotary_refuses_crossed_outputs_and_sizes_past_the_entry():
         with pytest.raises(ValueError):
             call()
     assert not out.any()
+
+
+@pytest.mark.parametrize("D,R", [(128, 64), (100, 50)])
+def test_rotary_one_sided(D, R):
+    """No key heads, no query heads, no heads; a norm of one of the two."""
+    announce(f"rotary one-sided D={D} R={R}")
+    gen = torch.Generator().manual_seed(D)
+    q, k = (torch.randn(5, h, D, generator=gen).bfloat16().to(DEV) for h in (3, 2))
+    table, pos = _table(16, R).to(DEV), torch.arange(5, device=DEV)
+    w = (torch.rand(D, generator=gen) + 0.5).bfloat16().to(DEV)
+    plain = rotary_qk(q.clone(), k.clone(), pos, table)
+    normed = rotary_qk(q.clone(), k.clone(), pos, table, q_weight=w, k_weight=w)
+    for kw, pick in (({"q_weight": w}, (normed[0], plain[1])), ({"k_weight": w}, (plain[0], normed[1]))):
+        got = rotary_qk(q.clone(), k.clone(), pos, table, **kw)
+        assert torch.equal(got[0], pick[0]) and torch.equal(got[1], pick[1])
+    got = rotary_qk(q.clone(), k[:, :0], pos, table)
+    assert torch.equal(got[0], plain[0]) and got[1].shape == (5, 0, D)
+    assert torch.equal(rotary_qk(q[:, :0], k.clone(), pos, table)[1], plain[1])
+    rotary_qk(q[:, :0], k[:, :0], pos, table)
+
+
+def test_rotary_head_major_views():
+    """Tensors stored [heads, T, D], read as [T, heads, D], in place and into
+    another order."""
+    announce("rotary head-major")
+    gen = torch.Generator().manual_seed(9)
+    q, k = (torch.randn(6, h, 64, generator=gen).bfloat16().to(DEV) for h in (4, 2))
+    table, pos = _table(16, 64).to(DEV), torch.arange(6, device=DEV)
+    want = rotary_qk(q.clone(), k.clone(), pos, table)
+    qh, kh = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k))
+    out = rotary_qk(qh, kh, pos, table, q_out=torch.empty_like(q, memory_format=torch.contiguous_format),
+                    k_out=torch.empty_like(k, memory_format=torch.contiguous_format))
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    rotary_qk(qh, kh, pos, table)
+    assert torch.equal(qh, want[0]) and torch.equal(kh, want[1])
