@@ -1,5 +1,5 @@
-// MXFP4 product for few tokens: the weights stream once, K split over the
-// waves of a block.
+// MXFP4 products for few tokens: the weights stream once, K split over the
+// waves of a block, or, for many weight rows, the rows.
 #pragma once
 
 #include "mxfp4_ring.h"
@@ -200,6 +200,156 @@ __global__ __launch_bounds__(1024) void mxfp4_decode_kernel(MxDecodeArgs d) {
     if (g.bias) s += bf16_to_f32(g.bias[n0 + n]);
     g.out[m * g.N + n0 + n] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(s));
   }
+#endif
+}
+
+// Many weight rows: one block per CU keeps the tokens in LDS ([tile][16 TG
+// rows][256 code bytes, chunk c of row r at c ^ r], then scales [tile][16 TG
+// rows][16]).  It owns weight rows in units of 4; its waves split them evenly and
+// walk them in chunks of at most 16 rows, all of K each, through private rings
+// of D slots, so no sum crosses waves and nothing is synchronized after the
+// start.  (Above, every block loads the tokens again, 16 bytes a cycle where the
+// lanes of a load lie on different rows: 16 tokens cost 4 us more than one at
+// 34816 x 5120.)  Bound: HBM.  MI355X: 16 x 34816 x 5120 18.3 us (5.2 TB/s; split
+// along K 21.7), 32 tokens 19.0 (64 x 64 ring 25.3); 16 x 51200 x 5120 25.2 us
+// (5.5 TB/s; 29.3), 32 tokens 26.4 (35.1).
+template <int TG, int D>
+__global__ __launch_bounds__(1024) void mxfp4_decode_shared_kernel(MxArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kOps = 5;  // vector memory operations per tile
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, grp = lane >> 4, waves = blockDim.x >> 6;
+  const int64_t units = (g.N + 3) / 4, parts = static_cast<int64_t>(gridDim.x) * waves;
+  const int64_t part = static_cast<int64_t>(blockIdx.x) * waves + wave;
+  const int64_t u0 = units * part / parts, u1 = units * (part + 1) / parts;
+  const int own = static_cast<int>(u1 - u0), chunks = (own + 3) / 4;
+  const int M = static_cast<int>(g.M), tiles = g.tiles;
+  const int64_t ld = static_cast<int64_t>(g.kb) * 16;
+  unsigned char* const tok = lds;
+  unsigned char* const tok_s = lds + tiles * (TG * kMxSlot);
+  unsigned char* const ring = tok_s + tiles * (TG * 256) + wave * (D * kMxSlot);
+  auto view = [](const void* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(scalar_ptr(const_cast<uint8_t*>(static_cast<const uint8_t*>(p))), 0,
+                                             __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), kBufferFlags);
+  };
+  uint32_t off[4];  // DMA instruction j: rows 4 j .. 4 j + 3, chunk c of row r at c ^ r
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = 4 * j + grp;
+    off[j] = static_cast<uint32_t>(row * ld + 16 * (r16 ^ row));
+  }
+  // chunk c of the wave: units [u0 + own c / chunks, u0 + own (c + 1) / chunks)
+  auto first = [&](int c) { return 4 * (u0 + static_cast<uint32_t>(own * c) / static_cast<uint32_t>(chunks)); };
+  // the next tile to load: tile it of chunk ic, weight rows n_in .. n_in + rows - 1
+  // (none behind the last chunk: every load reads zeros)
+  int ic = 0, it = 0, rows = 0;
+  int64_t n_in = 0;
+  auto enter = [&] {
+    const bool live = ic < chunks;
+    const int64_t end = live ? first(ic + 1) : 0;
+    n_in = live ? first(ic) : 0;
+    rows = static_cast<int>((end < g.N ? end : g.N) - n_in);
+  };
+  enter();
+  int sw[D];
+  auto issue = [&](int slot) {
+    const __amdgpu_buffer_rsrc_t w_rsrc = view(g.W + n_in * ld, rows * ld);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_ptr_t)(ring + slot * kMxSlot + j * 1024), 16, off[j], it * 256, 0,
+                                               kStreamAux);
+    const __amdgpu_buffer_rsrc_t sw_rsrc = view(g.sw + (it * g.N + n_in) * 16, rows * 16);
+    sw[slot] = __builtin_amdgcn_raw_buffer_load_b32(sw_rsrc, r16 * 16 + 4 * grp, 0, 0);
+    if (++it == tiles) {
+      it = 0;
+      ++ic;
+      enter();
+    }
+  };
+  const __amdgpu_buffer_rsrc_t a_rsrc = view(g.A, M * ld);
+  for (int t = wave; t < tiles; t += waves) {
+#pragma unroll
+    for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_ptr_t)(tok + (t * TG + tg) * kMxSlot + j * 1024), 16,
+                                                 static_cast<uint32_t>(off[j] + 16 * tg * ld), t * 256, 0, 0);
+    const __amdgpu_buffer_rsrc_t s_rsrc = view(g.sa + static_cast<int64_t>(t) * M * 16, M * 16);
+    if (lane < 16 * TG) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(s_rsrc, lane * 16, 0, 0);
+      *reinterpret_cast<v4i*>(tok_s + t * (TG * 256) + lane * 16) = __builtin_bit_cast(v4i, v);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < D; ++s) issue(s);
+  wait_vmcnt<D * kOps>();  // this wave's part of the tokens
+  __syncthreads();
+  v4f acc[TG] = {};
+  int c = 0, t = 0;
+  auto consume = [&](int slot) {
+    const unsigned char* const ws = ring + slot * kMxSlot + r16 * 256;
+    v4i w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const v4i*>(ws + 16 * ((8 * (j >> 1) + 2 * grp + (j & 1)) ^ r16));
+#pragma unroll
+    for (int tg = 0; tg < TG; ++tg) {
+      const unsigned char* const xs = tok + (t * TG + tg) * kMxSlot + r16 * 256;
+      const int s = *reinterpret_cast<const int*>(tok_s + (t * TG + tg) * 256 + r16 * 16 + 4 * grp);
+      v4i x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const v4i*>(xs + 16 * ((8 * (j >> 1) + 2 * grp + (j & 1)) ^ r16));
+      acc[tg] = mx_mma<0>(w[0], x[0], acc[tg], sw[slot], s);
+      acc[tg] = mx_mma<1>(w[1], x[1], acc[tg], sw[slot], s);
+      acc[tg] = mx_mma<2>(w[2], x[2], acc[tg], sw[slot], s);
+      acc[tg] = mx_mma<3>(w[3], x[3], acc[tg], sw[slot], s);
+    }
+  };
+  auto finish = [&] {  // chunk c is summed: a lane holds 4 columns of token r16
+    const int64_t n0 = first(c) + 4 * grp, end = first(c + 1), n1 = end < g.N ? end : g.N;
+    if (n0 < n1) {
+#pragma unroll
+      for (int tg = 0; tg < TG; ++tg) {
+        const int m = 16 * tg + r16;
+        uint16_t o[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          o[v] = __builtin_bit_cast(
+              uint16_t, static_cast<__bf16>(acc[tg][v] + (g.bias && n0 + v < n1 ? bf16_to_f32(g.bias[n0 + v]) : 0.0f)));
+        uint16_t* at = g.out + m * g.N + n0;
+        if (m < M) {
+          if (g.store >= 4) {
+            *reinterpret_cast<uint2*>(at) = make_uint2(o[0] | static_cast<uint32_t>(o[1]) << 16, o[2] | static_cast<uint32_t>(o[3]) << 16);
+          } else {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (n0 + v < n1) at[v] = o[v];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int tg = 0; tg < TG; ++tg) acc[tg] = v4f{};
+  };
+  const int items = chunks * tiles;
+  for (int i = 0; i < items; i += D) {
+#pragma unroll
+    for (int s = 0; s < D; ++s) {
+      wait_vmcnt<(D - 1) * kOps>();  // (loads retire in order; a chunk's stores only make it wait for more)
+      if (i + s < items) {
+        consume(s);
+        if (++t == tiles) {
+          finish();
+          t = 0;
+          ++c;
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // the slot's fragments are read before its refill
+      issue(s);
+    }
+  }
+  wait_vmcnt<0>();
 #endif
 }
 

@@ -54,8 +54,32 @@ constexpr int kNumMxRings = sizeof(kMxRings) / sizeof(kMxRings[0]);
 constexpr int kMxSplitCfg = 4, kMxMaxSplit = 16, kMxDecodeRows = 16;
 
 struct MxPlan {
-  int cfg, split;  // cfg < 0: the decode kernel
+  int cfg, split;  // cfg < 0: a decode kernel
 };
+
+// The decode kernel whose blocks keep the tokens in LDS: waves per block (0: the
+// others are faster) and ring slots per wave.  It pays from 96 weight rows per
+// CU on, for 8 tokens and more, up to 12 tiles of them (MI355X, us, this / the
+// other: 16 x 24576 x 5120 13.8 / 14.7, 32 rows 14.5 / 18.3; 8 x 34816 x 5120 18.5 /
+// 19.3; 16 x 40000 x 1024 7.3 / 10.3; but 32 x 16384 x 2048 6.8 / 6.5, 5 x 58208 x
+// 1568 15.4 / 13.7, 16 x 32768 x 8192 31 / 27; 14 random shapes within the rule 0.66
+// to 1.04 of the other's time).  As many waves as give each
+// chunks of 16 rows, with two slots where the LDS holds them (16 x 24576 x 5120,
+// 6 waves: two slots 13.8, one 14.3; 8 waves, 12 rows each: 13.9).
+struct MxSharedPlan {
+  int waves, depth;
+};
+constexpr int kMxSharedRows = 32;
+MxSharedPlan mx_shared_plan(int64_t M, int64_t N, int64_t K) {
+  const int64_t cus = device_cus(), tiles = mx_tiles(K);
+  // (chunks are counted in 32 bits)
+  if (M < 8 || M > kMxSharedRows || N < 96 * cus || N >= (1ll << 26) || tiles > 12) return {0, 0};
+  const int64_t rows = (N + cus - 1) / cus;
+  const int64_t room = (kLdsBytes - tiles * (M > 16 ? 2 : 1) * (kMxSlot + 256)) / kMxSlot;
+  const int64_t most = std::min<int64_t>(room, 16), chunks = (rows + 16 * most - 1) / (16 * most);
+  const int64_t waves = (rows + 16 * chunks - 1) / (16 * chunks);
+  return {static_cast<int>(waves), 2 * waves <= room ? 2 : 1};
+}
 
 thread_local int g_mx_cfg = -1, g_mx_split = 0;  // override of the calling thread (-1: automatic)
 
@@ -80,7 +104,7 @@ MxPlan mx_plan(int64_t M, int64_t N, int64_t K, bool may_split) {
     const bool split = may_split && g_mx_cfg == kMxSplitCfg && g_mx_split > 1 && g_mx_split <= tiles;
     return {g_mx_cfg, split ? g_mx_split : 1};
   }
-  if (M <= kMxDecodeRows) return {-1, 1};
+  if (M <= kMxDecodeRows || mx_shared_plan(M, N, K).waves > 0) return {-1, 1};
   MxPlan best{0, 1};
   double us = 1e30;
   for (int c = 0; c < kNumMxRings; ++c) {
@@ -176,6 +200,15 @@ int launch_decode(const MxDecodeArgs& d, const MxDecodePlan& p, hipStream_t st) 
   return check_launch("gemm_mxfp4");
 }
 
+template <int TG, int D>
+int launch_decode_shared(const MxArgs& g, int waves, hipStream_t st) {
+  constexpr auto kern = mxfp4_decode_shared_kernel<TG, D>;
+  if (const int rc = mx_lds_limit<kern>(kLdsBytes)) return rc;
+  const int lds = g.tiles * TG * (kMxSlot + 256) + waves * D * kMxSlot;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(device_cus())), dim3(64 * waves), lds, st, g);
+  return check_launch("gemm_mxfp4");
+}
+
 MxArgs mx_args(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, const void* bias, void* y,
                int64_t M, int64_t N, int64_t K) {
   // (16-byte stores go through a 32-bit view of a tile's output rows)
@@ -210,6 +243,10 @@ int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const
   MxArgs g = mx_args(A, sa, W, sw, bias, y, M, N, K);
   const MxPlan p = mx_plan(M, N, K, ws != nullptr);
   if (p.cfg < 0) {
+    if (const MxSharedPlan sp = mx_shared_plan(M, N, K); sp.waves > 0) {
+      if (M > 16) return sp.depth == 2 ? launch_decode_shared<2, 2>(g, sp.waves, st) : launch_decode_shared<2, 1>(g, sp.waves, st);
+      return sp.depth == 2 ? launch_decode_shared<1, 2>(g, sp.waves, st) : launch_decode_shared<1, 1>(g, sp.waves, st);
+    }
     const MxDecodePlan dp = mx_decode_plan(M, N, K);
     const MxDecodeArgs d{g, nullptr, 0, K, dp.per_wave};
     return dp.groups == 2 ? launch_decode<2, false>(d, dp, st) : launch_decode<1, false>(d, dp, st);

@@ -393,3 +393,71 @@ def test_gemm_rows_behind_the_last(M):
         buf = torch.full((M + 300, N), 3.0, dtype=torch.bfloat16, device=DEV)
         y = gemm_mxfp4(*a, *w, out=buf[:M])
         assert torch.equal(y, gemm_mxfp4(*a, *w)) and (buf[M:] == 3).all()
+
+
+MANY = 24576  # weight rows from which 8 to 32 tokens are kept on chip (256 compute units)
+
+
+@pytest.mark.parametrize("M", [7, 8, 16, 17, 32, 33])
+@pytest.mark.parametrize("N,K", [(MANY - 1, 32), (MANY, 32), (MANY + 1, 544), (MANY + 6, 1024), (MANY + 4, 500), (33000, 160)])
+def test_many_weight_rows(M, N, K):
+    """Few tokens on many weight rows, exact inputs; rows behind the last stay."""
+    announce(f"gemm_mxfp4 many rows M={M} N={N} K={K}")
+    a, av = _operand(M, K, seed=M)
+    w, wv = _operand(N, K, seed=N)
+    b = np.random.default_rng(N).integers(-8, 9, N) / 4
+    bias = torch.from_numpy(b).bfloat16().to(DEV)
+    buf = torch.full((M + 32, N), 3.0, dtype=torch.bfloat16, device=DEV)
+    for bb, bd in ((None, None), (b, bias)):
+        want, size = orc.product(av, wv, bb)
+        assert size.max() * 4 < 2**24
+        np.testing.assert_array_equal(f32(gemm_mxfp4(*a, *w, bd, out=buf[:M])).astype(np.float64), orc.round_bf16(want))
+        assert (buf[M:] == 3).all()
+    # an output whose rows are not 8-byte aligned
+    odd = torch.empty(M * N + 1, dtype=torch.bfloat16, device=DEV)[1:].view(M, N)
+    assert torch.equal(gemm_mxfp4(*a, *w, bias, out=odd), buf[:M])
+
+
+@pytest.mark.parametrize("M", [9, 16, 31])
+@pytest.mark.parametrize("N,K", [(34816, 5120), (51200, 5120), (40008, 6144), (40008, 6176), (70000, 1536)])
+def test_many_weight_rows_equal_a_tiling(tuning, M, N, K):
+    """Exact inputs (|sums| below 144 K < 2^22, multiples of 1/4): the bits of
+    the tile rings."""
+    announce(f"gemm_mxfp4 many rows M={M} N={N} K={K} against a tiling")
+    gen = torch.Generator().manual_seed(M + N)
+    ops = []
+    for rows in (M, N):
+        codes = torch.randint(0, 256, (rows, K // 2), dtype=torch.uint8, generator=gen)
+        ops += [codes.to(DEV), mxfp4_tile_scales(torch.randint(127, 129, (rows, K // 32), dtype=torch.uint8, generator=gen)).to(DEV)]
+    ops[1][0, M // 2, 3] = 255  # a NaN block reaches its row only
+    got = gemm_mxfp4(*ops)
+    tuning(2, 0)
+    want = gemm_mxfp4(*ops)
+    assert torch.isnan(want[M // 2]).all() and torch.isnan(got[M // 2]).all()
+    keep = [m for m in range(M) if m != M // 2]
+    assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("M", [16, 32])
+def test_many_weight_rows_on_streams_and_in_a_graph(M):
+    announce(f"gemm_mxfp4 many rows on streams and in a graph M={M}")
+    w, _ = _operand(MANY, 1024, seed=1)
+    xs = [_operand(M, 1024, seed=2 + i)[0] for i in range(3)]
+    want = [gemm_mxfp4(*x, *w) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(gemm_mxfp4(*xs[i % 3], *w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(got))
+    q, s = xs[0][0].clone(), xs[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = gemm_mxfp4(q, s, *w)
+    for i in (1, 2, 0, 2):
+        q.copy_(xs[i][0]), s.copy_(xs[i][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i])
