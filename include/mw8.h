@@ -491,6 +491,20 @@ int32_t mw8_gemm_act_mxfp4_supported(int64_t M, int64_t I, int64_t K);
 int32_t mw8_gemm_act_mxfp4_preferred(int64_t M, int64_t I, int64_t K);
 
 /*
+ * The gated MLP: y bf16 [M, N] = down(act(gate) * up) with gate_up [2I, H] (gate
+ * rows first) and down [N, I] quantized, of x bf16 [M, H] (row stride ldx) or,
+ * if x is NULL, of quantized rows q, s; the bits of its parts one by one.
+ * workspace: 16-byte aligned, at least _workspace_bytes(x == NULL, M, H, I, N) bytes
+ * (the rows between the launches); calls that share one must be ordered on
+ * one stream.  H, I <= 2^20.
+ */
+int mw8_gated_mlp_mxfp4(const void* x, int64_t ldx, const uint8_t* q, const uint8_t* s, const uint8_t* w_gate_up,
+                        const uint8_t* s_gate_up, const uint8_t* w_down, const uint8_t* s_down, int32_t act, void* y,
+                        int64_t M, int64_t H, int64_t I, int64_t N, void* workspace, size_t workspace_bytes,
+                        mw8_stream_t stream);
+size_t mw8_gated_mlp_mxfp4_workspace_bytes(int32_t quantized, int64_t M, int64_t H, int64_t I, int64_t N);
+
+/*
  * Rotary position embedding of q [T, hq, D] and k [T, hk, D] (token and head
  * strides ld / hd in elements, heads contiguous) into q_out / k_out (which
  * may be q / k): pair (a, b) of the first R elements of a head turns to

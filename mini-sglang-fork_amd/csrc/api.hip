@@ -90,6 +90,9 @@ int gemm_act_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t
                    int64_t, hipStream_t);
 int gemm_act_mxfp4_supported(int64_t, int64_t, int64_t);
 int gemm_act_mxfp4_preferred(int64_t, int64_t, int64_t);
+size_t gated_mlp_mxfp4_workspace_bytes(int, int64_t, int64_t, int64_t, int64_t);
+int gated_mlp_mxfp4(const void*, int64_t, const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*,
+                    const uint8_t*, int, void*, int64_t, int64_t, int64_t, int64_t, void*, size_t, hipStream_t);
 int rotary_qk(const void*, int64_t, int64_t, int, const void*, int64_t, int64_t, int, void*, int64_t, int64_t, void*,
               int64_t, int64_t, int, int, int, int, const void*, int, const float*, int64_t, const void*, const void*,
               float, int64_t, hipStream_t);
@@ -326,6 +329,16 @@ int mw8_linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const ui
 int mw8_gemm_act_mxfp4(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int32_t act, uint8_t* q,
                        uint8_t* s, int64_t M, int64_t I, int64_t K, mw8_stream_t st) {
   MW8_ENTRY(mw8::gemm_act_mxfp4(A, sa, W, sw, act, q, s, M, I, K, S(st)));
+}
+
+int mw8_gated_mlp_mxfp4(const void* x, int64_t ldx, const uint8_t* q, const uint8_t* s, const uint8_t* Wg, const uint8_t* sg,
+                        const uint8_t* Wd, const uint8_t* sd, int32_t act, void* y, int64_t M, int64_t H, int64_t I,
+                        int64_t N, void* ws, size_t ws_bytes, mw8_stream_t st) {
+  MW8_ENTRY(mw8::gated_mlp_mxfp4(x, ldx, q, s, Wg, sg, Wd, sd, act, y, M, H, I, N, ws, ws_bytes, S(st)));
+}
+
+size_t mw8_gated_mlp_mxfp4_workspace_bytes(int32_t quantized, int64_t M, int64_t H, int64_t I, int64_t N) {
+  return mw8::gated_mlp_mxfp4_workspace_bytes(quantized, M, H, I, N);
 }
 
 int32_t mw8_gemm_act_mxfp4_preferred(int64_t M, int64_t I, int64_t K) { return mw8::gemm_act_mxfp4_preferred(M, I, K); }

@@ -10,6 +10,8 @@
 namespace mw8 {
 
 int device_cus();
+int quant_mxfp4_bf16(const void*, int64_t, int64_t, int64_t, uint8_t*, uint8_t*, hipStream_t);
+int act_and_mul_quant_mxfp4_bf16(const void*, int64_t, int64_t, int, uint8_t*, uint8_t*, hipStream_t);
 
 namespace {
 
@@ -164,7 +166,7 @@ int run_ring(const MxArgs& g, int cfg, hipStream_t st) {
 // ------------------------------------------------------------------ decode
 // 16-row groups per block and 512-element tiles per wave.  Two row groups
 // share the tokens' fragments and leave N <= 32 x CUs one block per CU (MI355X,
-// us, one -> two groups: 16 x 34816 x 5120 24.3 -> 21.7, 16 x 5120 x 17408
+// us, one -> two groups: 16 x 16384 x 5120 12.1 -> 10.8, 16 x 5120 x 17408
 // 15.5 -> 12.8); few tokens and more rows than that are faster in single
 // groups (1 x 34816 x 5120 18.6 -> 17.6, 8 tokens 19.7 -> 19.2).  Four tiles
 // per wave, two where single groups have enough waves (1 x 34816 x 5120 18.3
@@ -309,10 +311,15 @@ int linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K) {
          mx_decode_lds(p, M, K, true) <= kLdsBytes;
 }
 
+// Rows that it can read: whole 16-byte vectors within a 32-bit view.
+static bool linear_takes(const void* x, int64_t ldx, int64_t M) {
+  return aligned_to(x, 16) && (M == 1 || (ldx % 8 == 0 && ldx < (1ll << 26)));
+}
+
 int linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_t* sw, const void* bias, void* y, int64_t M,
                       int64_t N, int64_t K, hipStream_t st) {
   MW8_REQUIRE(x && W && sw && y, kErrArg, "linear_mxfp4: null pointer");
-  MW8_REQUIRE(M >= 0 && N > 0 && K > 0 && ldx >= K && ldx < (1ll << 26), kErrShape,
+  MW8_REQUIRE(M >= 0 && N > 0 && K > 0 && ldx >= K && (M == 1 || ldx < (1ll << 26)), kErrShape,
               "linear_mxfp4: bad sizes M=%lld N=%lld K=%lld ldx=%lld", (long long)M, (long long)N, (long long)K, (long long)ldx);
   if (M == 0) return kOk;
   MW8_REQUIRE(linear_bf16_mxfp4_supported(M, N, K), kErrShape, "linear_mxfp4: M=%lld N=%lld K=%lld not supported",
@@ -321,9 +328,78 @@ int linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_
                   aligned_to(bias, 2),
               kErrAlign, "linear_mxfp4: x, its rows, W and sw need 16-byte, y and bias 2-byte alignment");
   const MxDecodePlan dp = mx_decode_plan(M, N, K);
-  const MxDecodeArgs d{mx_args(nullptr, nullptr, W, sw, bias, y, M, N, K), static_cast<const uint16_t*>(x), ldx, K,
+  const MxDecodeArgs d{mx_args(nullptr, nullptr, W, sw, bias, y, M, N, K), static_cast<const uint16_t*>(x), M == 1 ? K : ldx, K,
                        dp.per_wave};
   return dp.groups == 2 ? launch_decode<2, true>(d, dp, st) : launch_decode<1, true>(d, dp, st);
+}
+
+namespace {
+
+// The gated MLP's buffers between its launches, from the start of the workspace
+// (bytes; 256-byte aligned).
+struct MxMlpPlan {
+  bool act_in_product;
+  size_t xq, xs, gate_up, aq, as, part, part_bytes, total;
+};
+MxMlpPlan mx_mlp_plan(bool quantized, int64_t M, int64_t H, int64_t I, int64_t N) {
+  MxMlpPlan p{};
+  p.act_in_product = gemm_act_mxfp4_preferred(M, I, H) != 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = p.total;
+    p.total += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t m = static_cast<size_t>(M);
+  p.xq = take(quantized ? 0 : m * mx_blocks(H) * 16);
+  p.xs = take(quantized ? 0 : m * mx_tiles(H) * kMxTileBlocks);
+  p.gate_up = take(p.act_in_product ? 0 : m * I * 4);
+  p.aq = take(m * mx_blocks(I) * 16);
+  p.as = take(m * mx_tiles(I) * kMxTileBlocks);
+  p.part_bytes = std::max(p.act_in_product ? 0 : gemm_mxfp4_workspace_bytes(M, 2 * I, H), gemm_mxfp4_workspace_bytes(M, N, I));
+  p.part = take(p.part_bytes);
+  return p;
+}
+
+bool mx_mlp_sizes(int64_t M, int64_t H, int64_t I, int64_t N) {
+  return M >= 0 && H > 0 && I > 0 && N > 0 && M < (1ll << 31) && H <= (1ll << 20) && I <= (1ll << 20) && N < (1ll << 31);
+}
+
+}  // namespace
+
+size_t gated_mlp_mxfp4_workspace_bytes(int quantized, int64_t M, int64_t H, int64_t I, int64_t N) {
+  return M > 0 && mx_mlp_sizes(M, H, I, N) ? mx_mlp_plan(quantized != 0, M, H, I, N).total : 0;
+}
+
+int gated_mlp_mxfp4(const void* x, int64_t ldx, const uint8_t* q, const uint8_t* s, const uint8_t* Wg, const uint8_t* sg,
+                    const uint8_t* Wd, const uint8_t* sd, int act, void* y, int64_t M, int64_t H, int64_t I, int64_t N,
+                    void* ws, size_t ws_bytes, hipStream_t st) {
+  MW8_REQUIRE((x || (q && s)) && Wg && sg && Wd && sd && y, kErrArg, "gated_mlp_mxfp4: null pointer");
+  MW8_REQUIRE(act == 0 || act == 1, kErrArg, "gated_mlp_mxfp4: act must be 0 (silu) or 1 (gelu)");
+  MW8_REQUIRE(mx_mlp_sizes(M, H, I, N) && (!x || ldx >= H), kErrShape, "gated_mlp_mxfp4: bad sizes M=%lld H=%lld I=%lld N=%lld",
+              (long long)M, (long long)H, (long long)I, (long long)N);
+  if (M == 0) return kOk;
+  const MxMlpPlan p = mx_mlp_plan(!x, M, H, I, N);
+  MW8_REQUIRE(ws && ws_bytes >= p.total, kErrWorkspace, "gated_mlp_mxfp4: the workspace holds %zu of %zu bytes", ws ? ws_bytes : 0,
+              p.total);
+  MW8_REQUIRE(aligned_to(ws, 16), kErrAlign, "gated_mlp_mxfp4: the workspace needs 16-byte alignment");
+  auto* b = static_cast<uint8_t*>(ws);
+  void* part = p.part_bytes > 0 ? b + p.part : nullptr;
+  void* gu = b + p.gate_up;
+  const bool one = x && linear_takes(x, ldx, M) && linear_bf16_mxfp4_supported(M, 2 * I, H);
+  if (x && !one) {
+    if (const int rc = quant_mxfp4_bf16(x, M, H, ldx, b + p.xq, b + p.xs, st)) return rc;
+    q = b + p.xq;
+    s = b + p.xs;
+  }
+  if (p.act_in_product) {
+    if (const int rc = gemm_act_mxfp4(q, s, Wg, sg, act, b + p.aq, b + p.as, M, I, H, st)) return rc;
+  } else {
+    if (const int rc = one ? linear_bf16_mxfp4(x, ldx, Wg, sg, nullptr, gu, M, 2 * I, H, st)
+                           : gemm_mxfp4_bf16(q, s, Wg, sg, nullptr, gu, M, 2 * I, H, part, p.part_bytes, st))
+      return rc;
+    if (const int rc = act_and_mul_quant_mxfp4_bf16(gu, M, 2 * I, act, b + p.aq, b + p.as, st)) return rc;
+  }
+  return gemm_mxfp4_bf16(b + p.aq, b + p.as, Wd, sd, nullptr, y, M, N, I, part, p.part_bytes, st);
 }
 
 }  // namespace mw8

@@ -95,6 +95,8 @@ SIGNATURES = {
     "mw8_mxfp4_tuning_count": (_I32, []),
     "mw8_linear_bf16_mxfp4": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
     "mw8_gemm_act_mxfp4": (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P]),
+    "mw8_gated_mlp_mxfp4": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _I64, _I64, _P, c_size_t, _P]),
+    "mw8_gated_mlp_mxfp4_workspace_bytes": (c_size_t, [_I32, _I64, _I64, _I64, _I64]),
     "mw8_gemm_act_mxfp4_supported": (_I32, [_I64, _I64, _I64]),
     "mw8_gemm_act_mxfp4_preferred": (_I32, [_I64, _I64, _I64]),
     "mw8_linear_bf16_mxfp4_supported": (_I32, [_I64, _I64, _I64]),

@@ -36,8 +36,8 @@ def _tiles(K: int) -> int:
 
 
 def _empty(rows: int, K: int, like: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    codes = torch.empty((rows, _codes_width(K)), dtype=torch.uint8, device=like.device)
-    scale = torch.empty((_tiles(K), rows, 16), dtype=torch.uint8, device=like.device)
+    codes = torch.empty(rows, _codes_width(K), dtype=torch.uint8, device=like.device)
+    scale = torch.empty(_tiles(K), rows, 16, dtype=torch.uint8, device=like.device)
     return codes, scale
 
 
@@ -272,12 +272,9 @@ def gated_mlp_mxfp4(
     _one_gpu(x, w_gate_up, s_gate_up, w_down, s_down)
     _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "gated_mlp_mxfp4: x must be bf16 [..., H]")
     inter, N = _check_mlp(x.shape[-1], w_gate_up, s_gate_up, w_down, s_down, activation)
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if _fused_act(x2.shape[0], inter, x2.shape[1], x2):
-        codes, scale = gemm_act_mxfp4(*quant_mxfp4(_rows(x2)), w_gate_up, s_gate_up, activation)
-    else:
-        codes, scale = act_and_mul_quant_mxfp4(linear_mxfp4(x2, w_gate_up, s_gate_up), activation)
-    y = gemm_mxfp4(codes, scale, w_down, s_down)
+    x2 = _rows(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    M, H = x2.shape
+    y = _mlp(x2, H if M <= 1 else x2.stride(0), None, None, w_gate_up, s_gate_up, w_down, s_down, activation, M, H, inter, N)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
@@ -294,12 +291,8 @@ def gated_mlp_quantized_mxfp4(
     of [M, H], as ``rmsnorm_quant_mxfp4`` gives them): bf16 [M, H']."""
     _one_gpu(codes, scale, w_gate_up, s_gate_up, w_down, s_down)
     M, K = _check_operand("x", codes, scale, None), codes.shape[1] * 2
-    inter, _ = _check_mlp(K, w_gate_up, s_gate_up, w_down, s_down, activation)
-    if _fused_act(M, inter, K, codes):
-        codes, scale = gemm_act_mxfp4(codes, scale, w_gate_up, s_gate_up, activation)
-    else:
-        codes, scale = act_and_mul_quant_mxfp4(gemm_mxfp4(codes, scale, w_gate_up, s_gate_up), activation)
-    return gemm_mxfp4(codes, scale, w_down, s_down)
+    inter, N = _check_mlp(K, w_gate_up, s_gate_up, w_down, s_down, activation)
+    return _mlp(None, 0, codes, scale, w_gate_up, s_gate_up, w_down, s_down, activation, M, K, inter, N)
 
 
 def _check_mlp(K: int, w_gate_up, s_gate_up, w_down, s_down, activation: str) -> Tuple[int, int]:
@@ -307,15 +300,25 @@ def _check_mlp(K: int, w_gate_up, s_gate_up, w_down, s_down, activation: str) ->
     _need(activation in _ACT, f"unsupported activation {activation}")
     rows = _check_operand("gate_up", w_gate_up, s_gate_up, K)
     _need(rows > 0 and rows % 2 == 0, "gate_up: 2I rows")
-    return rows // 2, _check_operand("down", w_down, s_down, rows // 2)
+    N = _check_operand("down", w_down, s_down, rows // 2)
+    _need(N > 0, "down: at least one row")
+    return rows // 2, N
 
 
-def _fused_act(M: int, inter: int, K: int, like: torch.Tensor) -> bool:
-    """Whether gate_up, activation and quantizer run as one launch."""
-    if M <= 16:
-        return False
-    with _device_of(like):
-        return bool(load().mw8_gemm_act_mxfp4_preferred(M, inter, K))
+def _mlp(x, ldx: int, codes, scale, w_gate_up, s_gate_up, w_down, s_down, activation: str, M: int, H: int, inter: int,
+         N: int) -> torch.Tensor:
+    """The MLP's launches in one call (an eager call of each is bound by host
+    time in decode batches: 4 launches 35 us one by one)."""
+    like, lib = w_down, load()
+    y = torch.empty(M, N, dtype=torch.bfloat16, device=like.device)
+    if M > 0:
+        with _device_of(like):
+            need = lib.mw8_gated_mlp_mxfp4_workspace_bytes(x is None, M, H, inter, N)
+            ws = _call_workspace(need, like)
+            check(lib.mw8_gated_mlp_mxfp4(_ptr(x), ldx, _ptr(codes), _ptr(scale), w_gate_up.data_ptr(), s_gate_up.data_ptr(),
+                                          w_down.data_ptr(), s_down.data_ptr(), _ACT[activation], y.data_ptr(), M, H, inter, N,
+                                          _ptr(ws), need, _stream(like)))
+    return y
 
 
 __all__ = [

@@ -461,3 +461,48 @@ def test_many_weight_rows_on_streams_and_in_a_graph(M):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want[i])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,H,I,N", [(1, 512, 768, 512), (3, 1000, 500, 72), (8, 512, 12320, 264), (16, 2048, 768, 2048),
+                                     (20, 512, 12320, 264), (64, 512, 4096, 512), (300, 1024, 1056, 1000), (2100, 512, 3200, 512)])
+def test_gated_mlp_equals_its_parts(act, M, H, I, N):
+    """One call, of rows as they lie and of quantized ones: the bits of
+    quantizer, product, activation + quantizer and product."""
+    from minisgl_amd.kernel import act_and_mul_quant_mxfp4, gated_mlp_quantized_mxfp4
+
+    announce(f"gated_mlp_mxfp4 M={M} H={H} I={I} N={N} {act} against its parts")
+    gen = torch.Generator().manual_seed(M + I)
+    w1, _ = _operand(2 * I, H, seed=1, low=118, high=121)
+    w2, _ = _operand(N, I, seed=2, low=118, high=121)
+    wide = torch.randn(M, H + 8, generator=gen).bfloat16().to(DEV)
+    for x in (wide[:, :H].contiguous(), wide[:, 8:], wide[:, 3 : H + 3]):
+        q = quant_mxfp4(x)
+        want = gemm_mxfp4(*act_and_mul_quant_mxfp4(linear_mxfp4(x, *w1), act), *w2)
+        assert torch.equal(gated_mlp_mxfp4(x, *w1, *w2, act), want)
+        if H % 32 == 0:
+            want = gemm_mxfp4(*act_and_mul_quant_mxfp4(gemm_mxfp4(*q, *w1), act), *w2)
+            assert torch.equal(gated_mlp_quantized_mxfp4(*q, *w1, *w2, act), want)
+
+
+def test_gated_mlp_workspace():
+    """The C entry stays inside the workspace it asks for, and refuses a
+    smaller one."""
+    from minisgl_amd.kernel import load
+    from minisgl_amd.kernel.lib import check
+
+    lib = load()
+    announce("gated_mlp_mxfp4 workspace")
+    w1, _ = _operand(2 * 4096, 512, seed=1, low=118, high=121)
+    w2, _ = _operand(512, 4096, seed=2, low=118, high=121)
+    for M in (1, 16, 64, 300, 2100):
+        x = torch.randn(M, 512, generator=torch.Generator().manual_seed(M)).bfloat16().to(DEV)
+        need = lib.mw8_gated_mlp_mxfp4_workspace_bytes(0, M, 512, 4096, 512)
+        ws = torch.full((need + 4096,), 7, dtype=torch.uint8, device=DEV)
+        y = torch.empty(M, 512, dtype=torch.bfloat16, device=DEV)
+        args = (x.data_ptr(), 512, None, None, w1[0].data_ptr(), w1[1].data_ptr(), w2[0].data_ptr(), w2[1].data_ptr(), 0,
+                y.data_ptr(), M, 512, 4096, 512, ws.data_ptr())
+        st = torch.cuda.current_stream().cuda_stream
+        assert lib.mw8_gated_mlp_mxfp4(*args, need - 1, st) != 0
+        check(lib.mw8_gated_mlp_mxfp4(*args, need, st))
+        assert (ws[need:] == 7).all() and torch.equal(y, gated_mlp_mxfp4(x, *w1, *w2))

@@ -126,6 +126,23 @@ def test_launch_limits():
     assert lib.mw8_act_and_mul_quant_mxfp4_bf16(p, 4 * rows, 64, 0, p, p, None) == 2
 
 
+def test_gated_mlp_refusals():
+    lib = load()
+    p = ctypes.c_void_p(4096)
+
+    def call(x=p, ldx=64, q=None, s=None, w=p, act=0, y=p, M=1, H=64, I=32, N=16, ws=p, ws_bytes=1 << 20):
+        return lib.mw8_gated_mlp_mxfp4(x, ldx, q, s, w, p, p, p, act, y, M, H, I, N, ws, ws_bytes, None)
+
+    assert call(M=0) == 0 and call(M=0, x=None, q=p, s=p) == 0
+    assert call(x=None) == 1 and call(x=None, q=p) == 1 and call(w=None) == 1 and call(y=None) == 1 and call(act=2) == 1
+    assert call(ldx=63) == 2 and call(H=0) == 2 and call(I=0) == 2 and call(N=0) == 2 and call(M=-1) == 2
+    assert call(I=(1 << 20) + 1) == 2 and call(M=1 << 31) == 2
+    need = lib.mw8_gated_mlp_mxfp4_workspace_bytes(0, 1, 64, 32, 16)
+    assert need > 0 and call(ws_bytes=need - 1) == call(ws=None) != 0
+    assert call(ws=ctypes.c_void_p(4100), ws_bytes=need) == 3
+    assert lib.mw8_gated_mlp_mxfp4_workspace_bytes(0, 0, 64, 32, 16) == 0
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     w, s = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(1, 8, 16, dtype=torch.uint8)
