@@ -335,7 +335,14 @@ __global__ __launch_bounds__(TPR > 0 ? kBlock : 64 * kMaxWaves) void rmsnorm_row
       for (int j = 0; j < 4; ++j) {
         const float y0 = (bf16_lo(v[i].w[j]) * r) * bf16_lo(wv.w[j]);
         const float y1 = (bf16_hi(v[i].w[j]) * r) * bf16_hi(wv.w[j]);
-        v[i].w[j] = static_cast<uint32_t>(f32_to_bf16(y0)) | (static_cast<uint32_t>(f32_to_bf16(y1)) << 16);
+        if constexpr (QUANT == kMxfp4) {  // (the same rounding in one instruction)
+#if defined(__HIP_DEVICE_COMPILE__)
+          const mx_bf16x2 y = {static_cast<__bf16>(y0), static_cast<__bf16>(y1)};
+          v[i].w[j] = __builtin_bit_cast(uint32_t, y);
+#endif
+        } else {
+          v[i].w[j] = static_cast<uint32_t>(f32_to_bf16(y0)) | (static_cast<uint32_t>(f32_to_bf16(y1)) << 16);
+        }
       }
       if constexpr (QUANT == kInt8) m = absmax8(v[i], m);
     }
