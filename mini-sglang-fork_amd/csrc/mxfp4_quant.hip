@@ -60,8 +60,8 @@ __global__ __launch_bounds__(kMxThreads) void quant_mxfp4_kernel(const uint16_t*
       const U16x8 up = mx_load8<VEC>(x + r * ldx + K, k, K);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const mx_bf16x2 a = {static_cast<__bf16>(act_fn<ACT>(bf16_lo(v[u].w[j])) * bf16_lo(up.w[j])),
-                             static_cast<__bf16>(act_fn<ACT>(bf16_hi(v[u].w[j])) * bf16_hi(up.w[j]))};
+        const mx_bf16x2 a = {static_cast<__bf16>(mx_act_fn<ACT>(bf16_lo(v[u].w[j])) * bf16_lo(up.w[j])),
+                             static_cast<__bf16>(mx_act_fn<ACT>(bf16_hi(v[u].w[j])) * bf16_hi(up.w[j]))};
         v[u].w[j] = __builtin_bit_cast(uint32_t, a);
       }
     }

@@ -414,7 +414,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_ring_kernel(MxArgs g) {
             for (int k = 0; k < 2; ++k) {
               const float gate = static_cast<float>(static_cast<__bf16>(acc[i][j][2 * v + k]));
               const float up = static_cast<float>(static_cast<__bf16>(acc[i][j + kFN / 2][2 * v + k]));
-              a[k] = act_fn<kAct>(gate) * up;
+              a[k] = mx_act_fn<kAct>(gate) * up;
             }
             const mx_bf16x2 p = {static_cast<__bf16>(a[0]), static_cast<__bf16>(a[1])};
             (v < 4 ? lo.w[v] : hi.w[v - 4]) = __builtin_bit_cast(uint32_t, p);
