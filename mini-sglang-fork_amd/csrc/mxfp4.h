@@ -92,7 +92,10 @@ __device__ __forceinline__ uint32_t mx_quad_max(uint32_t m) {
 // 129 us; with erfcf 215, with 1 + erff 166; silu 105.
 template <int ACT>
 __device__ __forceinline__ float mx_act_fn(float g) {
-  if constexpr (ACT == 0) return act_fn<0>(g);  // silu
+  // silu: to zero from g = -87.3 down (below 2^-119; the reciprocal of e^87.3 is
+  // subnormal.  Halving the exponent there kept it, for 2 to 17% more time: 2080 x
+  // 25600 40.0 -> 46.9 us, in the product's epilogue 290 -> 298)
+  if constexpr (ACT == 0) return act_fn<0>(g);
   const float a = __builtin_fabsf(g), t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.0f));
   float q = 0.0359320343f;
   q = __builtin_fmaf(q, t, -0.158277139f);

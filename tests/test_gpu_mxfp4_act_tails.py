@@ -8,6 +8,8 @@ moves e^(-g^2 / 2) by g^2 / 2 at most; the exponential itself 1, the reciprocal 
 argument 1.5 (h grows no faster than the reciprocal), the polynomial 1.2 with its
 fit and 1/2 for each of 7 steps on partial sums of at most 1.5 times the result, three
 products 1.5, the product with up 1/2: delta = (g^2 + 19) 2^-23 is more than that.
+silu's e^-g has an exponent |g| / ln 2 off by 2^-23 of itself, |g| steps of the
+result; the exponential 1, the reciprocal and its argument 1.5, products 1: delta = (|g| + 8) 2^-23.
 The bf16 rounding adds 2^-8, and half a spacing of the code the rest."""
 
 import numpy as np
@@ -62,6 +64,13 @@ def test_gelu_tail():
     _check(x, "gelu", (f32(x).astype(np.float64)[:, :256] ** 2 + 19) * 2.0**-23)
 
 
+def test_silu_tail():
+    """Down to where the reciprocal leaves fp32's normal range (2^-126, g = -87.3)."""
+    announce("act_and_mul_quant_mxfp4 silu tail")
+    x = _tail(-87.0, -0.5, 2)
+    _check(x, "silu", (np.abs(f32(x).astype(np.float64)[:, :256]) + 8) * 2.0**-23)
+
+
 def _rows_of_gates(count, value, N, seed):
     """Quantized A [M, 64] of ones in the first count[m] columns, zeros behind,
     and W [2 N, 64]: gate rows `value`, up rows random levels.  So the gates of
@@ -84,4 +93,13 @@ def test_fused_gelu_tail_equals_its_parts(N):
     ops = _rows_of_gates([m % 27 for m in range(300)], -0.5, N, seed=N)
     want = act_and_mul_quant_mxfp4(gemm_mxfp4(*ops), "gelu")
     got = gemm_act_mxfp4(*ops, "gelu")
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("N", [64, 288])
+def test_fused_silu_tail_equals_its_parts(N):
+    announce(f"gemm_act_mxfp4 silu tail N={N}")
+    ops = _rows_of_gates([m % 30 for m in range(300)], -3.0, N, seed=N)
+    want = act_and_mul_quant_mxfp4(gemm_mxfp4(*ops), "silu")
+    got = gemm_act_mxfp4(*ops, "silu")
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
