@@ -29,6 +29,26 @@ from .base import BaseOP
 from .norm import _rows
 
 
+def _bf16_with_codes_of(w: torch.Tensor) -> torch.Tensor:
+    """bf16 values that quantize to the codes and scales of the float tensor w:
+    truncated, the last bit set where anything was dropped.  That keeps every
+    exponent, so the scales, and the side of every midpoint between two
+    levels (its last bf16 bit is 0).  Rounding to nearest would put 1.2500001 on
+    the midpoint 1.25 and from there on the wrong level.  Past fp32's range:
+    infinity."""
+    if w.dtype == torch.bfloat16:
+        return w
+    if w.dtype in (torch.float16, torch.float32):
+        bits = w.float().view(torch.int32)
+    else:  # the same step from 64 bits to 32
+        w = w.double()
+        v = w.float()
+        near = v.double()
+        bits = v.view(torch.int32) - ((near.abs() > w.abs()) & v.isfinite()).int()
+        bits |= ((near != w) & ~v.isinf()).int()
+    return ((bits >> 16) | ((bits & 0xFFFF) != 0).int()).to(torch.int16).view(torch.bfloat16)
+
+
 class LinearMXFP4(BaseOP):
     """``output_size`` a number of rows, or the list of a merged layer's."""
 
@@ -48,10 +68,11 @@ class LinearMXFP4(BaseOP):
         return gemm_mxfp4(codes, scale, self.weight, self.weight_scale, self.bias)
 
     def load_float_weight(self, w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
-        """Quantize a float [N, K] weight on the device into this layer."""
+        """Quantize a float [N, K] weight (any float type, one rounding) on the
+        device into this layer; the bias is rounded to bf16."""
         if w.shape != (self.output_size, self.input_size):
             raise ValueError(f"weight {tuple(w.shape)}, expected {(self.output_size, self.input_size)}")
-        self.weight, self.weight_scale = quant_mxfp4(w.to(torch.bfloat16).contiguous())
+        self.weight, self.weight_scale = quant_mxfp4(_bf16_with_codes_of(w).contiguous())
         self._load_bias(bias)
 
     def load_mxfp4_weight(self, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
