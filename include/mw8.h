@@ -506,13 +506,15 @@ size_t mw8_gated_mlp_mxfp4_workspace_bytes(int32_t quantized, int64_t M, int64_t
 
 /*
  * Rotary position embedding of q [T, hq, D] and k [T, hk, D] (token and head
- * strides ld / hd in elements, heads contiguous) into q_out / k_out (which
- * may be q / k): pair (a, b) of the first R elements of a head turns to
- * (a c - b s, b c + a s) with c, s from table fp32 [P, R] (R / 2 cosines,
- * then R / 2 sines) at the token's position; pairs are (i, R / 2 + i), or
- * (2 i, 2 i + 1) if interleaved.  q_weight / k_weight [D] (or NULL): per-head
- * RMSNorm first.  dtype 0 bf16, 1 fp16, 2 fp32; positions int32, or int64 if
- * pos64; a negative position leaves its rows, one >= P gives NaN.  D <= 8192.
+ * strides ld / hd in elements, heads contiguous) into q_out / k_out: pair
+ * (a, b) of the first R elements of a head turns to (a c - b s, b c + a s) with
+ * c, s from table fp32 [P, R] (R / 2 cosines, then R / 2 sines) at the token's
+ * position; pairs are (i, R / 2 + i), or (2 i, 2 i + 1) if interleaved.
+ * q_weight / k_weight [D] (or NULL): per-head RMSNorm first.  dtype 0 bf16, 1
+ * fp16, 2 fp32; positions int32, or int64 if pos64; a negative position leaves
+ * its rows, one >= P gives NaN.  D <= 8192.  q_out may be q with its strides,
+ * k_out k; else the rows of an output must share no memory with each other
+ * (MW8_ERR_SHAPE), the other output or an input (MW8_ERR_ARG).
  * Replaces apply_rope_with_cos_sin_cache_inplace
  * (python/minisgl/layers/rotary.py:35-52) and the per-head norms before it
  * (python/minisgl/layers/attention.py:49-53).

@@ -8,6 +8,7 @@
 // square and multiplied by the weight.  Everything is fp32 between the load
 // and the one rounding at the store.
 #include "mw8_common.h"
+#include "row_overlap.h"
 
 namespace mw8 {
 
@@ -244,6 +245,31 @@ int launch_rotary(const RotArgs& a, bool inter, hipStream_t st) {
   return check_launch("rotary_qk");
 }
 
+// Blocks write one token's (or head's) rows while others read theirs, so an
+// output may share memory with nothing but the input that it replaces.
+int check_rotary_overlap(const RotArgs& a, unsigned size) {
+  auto rows = [&](const void* p, int64_t ld, int64_t hd, int heads) {
+    const int64_t b = size;
+    return RowSet{p, a.D * b, a.T, ld * b, heads, hd * b};
+  };
+  const RowSet q = rows(a.q, a.q_ld, a.q_hd, a.hq), k = rows(a.k, a.k_ld, a.k_hd, a.hk);
+  const RowSet qo = rows(a.q_out, a.qo_ld, a.qo_hd, a.hq), ko = rows(a.k_out, a.ko_ld, a.ko_hd, a.hk);
+  auto same = [](const RowSet& x, const RowSet& y) {
+    return x.p == y.p && (x.n_outer == 1 || x.outer == y.outer) && (x.n_inner == 1 || x.inner == y.inner);
+  };
+  MW8_REQUIRE((row_set_empty(qo) || rows_apart(qo)) && (row_set_empty(ko) || rows_apart(ko)), kErrShape,
+              "rotary_qk: output rows must not overlap");
+  MW8_REQUIRE(!row_sets_meet(qo, ko), kErrArg, "rotary_qk: q_out and k_out must not overlap");
+  MW8_REQUIRE((same(qo, q) || !row_sets_meet(qo, q)) && (same(ko, k) || !row_sets_meet(ko, k)), kErrArg,
+              "rotary_qk: an output that is not its input must not overlap it");
+  MW8_REQUIRE(!row_sets_meet(qo, k) && !row_sets_meet(ko, q), kErrArg, "rotary_qk: q_out and k, k_out and q must not overlap");
+  for (const RowSet& r : {one_row(a.pos, a.T * (a.pos64 ? 8 : 4)), one_row(a.table, a.P * a.R * 4),
+                          one_row(a.qw, static_cast<int64_t>(a.D) * size), one_row(a.kw, static_cast<int64_t>(a.D) * size)})
+    MW8_REQUIRE(!row_sets_meet(qo, r) && !row_sets_meet(ko, r), kErrArg,
+                "rotary_qk: the outputs must not overlap positions, table or weights");
+  return kOk;
+}
+
 }  // namespace
 
 int rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int hq, const void* k, int64_t k_ld, int64_t k_hd, int hk,
@@ -269,6 +295,7 @@ int rotary_qk(const void* q, int64_t q_ld, int64_t q_hd, int hq, const void* k, 
               kErrAlign, "rotary_qk: tensors must be aligned to their elements");
   const RotArgs a{q, k, q_out, k_out, q_ld, q_hd, k_ld, k_hd, qo_ld, qo_hd, ko_ld, ko_hd, pos, table,
                   qw, kw, eps, T, P, hq, hk, D, R, pos64};
+  if (const int rc = check_rotary_overlap(a, size)) return rc;
   if (dtype == 0) return launch_rotary<__bf16>(a, interleaved != 0, st);
   if (dtype == 1) return launch_rotary<_Float16>(a, interleaved != 0, st);
   return launch_rotary<float>(a, interleaved != 0, st);

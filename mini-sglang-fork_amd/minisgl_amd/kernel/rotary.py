@@ -55,7 +55,8 @@ def rotary_qk(
 
     A token whose position is negative is padding: its output rows stay as
     they are.  One past the table turns to NaN.  Outputs may be the inputs
-    themselves; otherwise no output may overlap an input or the other."""
+    themselves; otherwise no output may overlap an input or the other (views
+    of one buffer that share no element are fine); the library refuses it."""
     _one_gpu(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
     _need(q.dtype in _DTYPE and k.dtype == q.dtype, "q and k: bf16, fp16 or fp32, the same")
     _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
