@@ -426,7 +426,9 @@ int mw8_moe_sum_reduce_bf16(const void* in, int64_t M, int32_t k, int64_t H, voi
  * Quantizer: e = floor(log2(amax)) - 2 clamped to [-127, 127] (amax = 0: -127),
  * elements rounded to nearest even, saturating at 6; a block with NaN or an
  * infinity gets byte 255.  No reference counterpart (the reference has no
- * quantized path); the entries stand where their int8 namesakes stand.
+ * quantized path); the entries stand where their int8 namesakes stand.  An
+ * output or workspace must share no memory with an input, another output or the
+ * workspace (MW8_ERR_ARG) but where an entry says so.
  */
 
 /* x bf16 [M, K] (row stride ldx >= K elements, any K) -> q, s.  x 2-byte, q 4-byte aligned
@@ -438,7 +440,8 @@ int mw8_quant_mxfp4_bf16(const void* x, int64_t M, int64_t K, int64_t ldx, uint8
 int mw8_act_and_mul_quant_mxfp4_bf16(const void* x, int64_t R, int64_t two_d, int32_t act, uint8_t* q, uint8_t* s,
                                      mw8_stream_t stream);
 
-/* As mw8_rmsnorm_quant_bf16 (residual updated in place, y optional), quantized to q, s; H % 8 == 0, H <= 32768. */
+/* As mw8_rmsnorm_quant_bf16 (residual updated in place, y optional and may be x), quantized to q, s; H % 8 == 0,
+ * H <= 32768. */
 int mw8_rmsnorm_quant_mxfp4_bf16(const void* x, void* residual, const void* weight, float eps, int64_t M, int64_t H,
                                  uint8_t* q, uint8_t* s, void* y, mw8_stream_t stream);
 

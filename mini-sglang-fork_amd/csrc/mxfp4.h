@@ -23,6 +23,7 @@
 #pragma once
 
 #include "mw8_common.h"
+#include "row_overlap.h"
 
 namespace mw8 {
 
@@ -32,6 +33,9 @@ constexpr int kMxTileBlocks = 16;
 
 MW8_HD int64_t mx_blocks(int64_t k) { return (k + kMxBlock - 1) / kMxBlock; }
 MW8_HD int64_t mx_tiles(int64_t k) { return (k + kMxTile - 1) / kMxTile; }
+// code and scale bytes of a quantized matrix as memory
+inline RowSet mx_codes_mem(const void* p, int64_t rows, int64_t k) { return one_row(p, rows * mx_blocks(k) * 16); }
+inline RowSet mx_scales_mem(const void* p, int64_t rows, int64_t k) { return one_row(p, rows * mx_tiles(k) * kMxTileBlocks); }
 // byte of block b (0..15) of a 512-element tile within its 16 scale bytes
 MW8_HD int mx_scale_pos(int b) { return ((b >> 1) & 3) * 4 + (b >> 3) * 2 + (b & 1); }
 

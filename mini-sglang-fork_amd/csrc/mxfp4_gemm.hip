@@ -242,6 +242,9 @@ int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const
                   aligned_to(bias, 2) && aligned_to(ws, 16),
               kErrAlign, "gemm_mxfp4: A, sa, W, sw and the workspace need 16-byte, y and bias 2-byte alignment");
   if (M == 0) return kOk;
+  MW8_REQUIRE(!any_meet({one_row(y, M * N * 2)}, {mx_codes_mem(A, M, K), mx_scales_mem(sa, M, K), mx_codes_mem(W, N, K),
+                                                 mx_scales_mem(sw, N, K), one_row(bias, N * 2)}),
+              kErrArg, "gemm_mxfp4: y must not overlap an input");
   MxArgs g = mx_args(A, sa, W, sw, bias, y, M, N, K);
   const MxPlan p = mx_plan(M, N, K, ws != nullptr);
   if (p.cfg < 0) {
@@ -256,6 +259,10 @@ int gemm_mxfp4_bf16(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const
   if (p.split > 1) {
     const size_t need = static_cast<size_t>(p.split) * M * N * 4;
     MW8_REQUIRE(ws_bytes >= need, kErrWorkspace, "gemm_mxfp4: the workspace holds %zu of %zu bytes", ws_bytes, need);
+    MW8_REQUIRE(!any_meet({one_row(ws, static_cast<int64_t>(need))},
+                          {one_row(y, M * N * 2), mx_codes_mem(A, M, K), mx_scales_mem(sa, M, K), mx_codes_mem(W, N, K),
+                           mx_scales_mem(sw, N, K), one_row(bias, N * 2)}),
+                kErrArg, "gemm_mxfp4: the workspace must not overlap y or an input");
     g.part = static_cast<float*>(ws);
     g.split = p.split;
   }
@@ -294,6 +301,9 @@ int gemm_act_mxfp4(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const 
               (long long)I, (long long)K);
   MW8_REQUIRE(aligned_to(A, 16) && aligned_to(W, 16) && aligned_to(sa, 16) && aligned_to(sw, 16) && aligned_to(q, 8), kErrAlign,
               "gemm_act_mxfp4: A, sa, W and sw need 16-byte and q 8-byte alignment");
+  MW8_REQUIRE(!any_meet({mx_codes_mem(q, M, I), mx_scales_mem(s, M, I)},
+                        {mx_codes_mem(A, M, K), mx_scales_mem(sa, M, K), mx_codes_mem(W, 2 * I, K), mx_scales_mem(sw, 2 * I, K)}),
+              kErrArg, "gemm_act_mxfp4: q and s must not overlap each other or an input");
   MxArgs g = mx_args(A, sa, W, sw, nullptr, nullptr, M, 2 * I, K);
   g.q = q;
   g.s = s;
@@ -327,6 +337,9 @@ int linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_
   MW8_REQUIRE(aligned_to(x, 16) && (M == 1 || ldx % 8 == 0) && aligned_to(W, 16) && aligned_to(sw, 16) && aligned_to(y, 2) &&
                   aligned_to(bias, 2),
               kErrAlign, "linear_mxfp4: x, its rows, W and sw need 16-byte, y and bias 2-byte alignment");
+  MW8_REQUIRE(!any_meet({one_row(y, M * N * 2)}, {RowSet{x, 2 * K, M, 2 * ldx, 1, 0}, mx_codes_mem(W, N, K),
+                                                 mx_scales_mem(sw, N, K), one_row(bias, N * 2)}),
+              kErrArg, "linear_mxfp4: y must not overlap an input");
   const MxDecodePlan dp = mx_decode_plan(M, N, K);
   const MxDecodeArgs d{mx_args(nullptr, nullptr, W, sw, bias, y, M, N, K), static_cast<const uint16_t*>(x), M == 1 ? K : ldx, K,
                        dp.per_wave};
@@ -382,6 +395,12 @@ int gated_mlp_mxfp4(const void* x, int64_t ldx, const uint8_t* q, const uint8_t*
   MW8_REQUIRE(ws && ws_bytes >= p.total, kErrWorkspace, "gated_mlp_mxfp4: the workspace holds %zu of %zu bytes", ws ? ws_bytes : 0,
               p.total);
   MW8_REQUIRE(aligned_to(ws, 16), kErrAlign, "gated_mlp_mxfp4: the workspace needs 16-byte alignment");
+  const RowSet none = one_row(nullptr, 0);
+  MW8_REQUIRE(!any_meet({one_row(y, M * N * 2), one_row(ws, static_cast<int64_t>(p.total))},
+                        {x ? RowSet{x, 2 * H, M, 2 * ldx, 1, 0} : none, x ? none : mx_codes_mem(q, M, H),
+                         x ? none : mx_scales_mem(s, M, H), mx_codes_mem(Wg, 2 * I, H), mx_scales_mem(sg, 2 * I, H),
+                         mx_codes_mem(Wd, N, I), mx_scales_mem(sd, N, I)}),
+              kErrArg, "gated_mlp_mxfp4: y and the workspace must not overlap each other or an input");
   auto* b = static_cast<uint8_t*>(ws);
   void* part = p.part_bytes > 0 ? b + p.part : nullptr;
   void* gu = b + p.gate_up;

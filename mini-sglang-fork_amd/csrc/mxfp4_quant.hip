@@ -130,6 +130,9 @@ int launch_quant(const char* what, const uint16_t* x, int64_t ldx, int64_t M, in
   const int U = M * mx_tiles(K) >= 16384 ? 4 : 1;
   const unsigned grid = mx_grid(M, K, U);
   MW8_REQUIRE(grid > 0, kErrShape, "%s: M=%lld x K=%lld too large", what, (long long)M, (long long)K);
+  MW8_REQUIRE(!any_meet({mx_codes_mem(q, M, K), mx_scales_mem(s, M, K)},
+                        {RowSet{x, (ACT >= 0 ? 4 : 2) * K, M, 2 * ldx, 1, 0}}),
+              kErrArg, "%s: q and s must not overlap each other or x", what);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(grid), dim3(kMxThreads), 0, st, x, ldx, M, K, q, s); };
   if (U == 4) {
     if (vec) go(quant_mxfp4_kernel<4, true, ACT>);
@@ -174,6 +177,8 @@ int dequant_mxfp4_bf16(const uint8_t* q, const uint8_t* s, int64_t M, int64_t K,
   if (M == 0) return kOk;
   const unsigned grid = mx_grid(M, K, 1);
   MW8_REQUIRE(grid > 0, kErrShape, "dequant_mxfp4: M=%lld x K=%lld too large", (long long)M, (long long)K);
+  MW8_REQUIRE(!any_meet({one_row(y, M * K * 2)}, {mx_codes_mem(q, M, K), mx_scales_mem(s, M, K)}), kErrArg,
+              "dequant_mxfp4: y must not overlap q or s");
   auto* yb = static_cast<uint16_t*>(y);
   if (K % 8 == 0 && aligned_to(y, 16))
     hipLaunchKernelGGL(dequant_mxfp4_kernel<true>, dim3(grid), dim3(kMxThreads), 0, st, q, s, M, K, yb);

@@ -656,6 +656,11 @@ int rmsnorm_quant_mxfp4_bf16(const void* x, void* residual, const void* weight, 
   MW8_REQUIRE(aligned16(x) && aligned16(weight) && (reinterpret_cast<uintptr_t>(q) & 3u) == 0 &&
                   (!residual || aligned16(residual)) && (!y || aligned16(y)),
               kErrAlign, "rmsnorm_quant_mxfp4: x/residual/weight/y need 16-byte and q 4-byte alignment");
+  MW8_REQUIRE(H <= 32768, kErrShape, "rmsnorm_quant_mxfp4: H=%lld exceeds the register-resident limit 32768", (long long)H);
+  const RowSet xm = one_row(x, M * H * 2), ym = one_row(y, M * H * 2), rm = one_row(residual, M * H * 2),
+               wm = one_row(weight, H * 2), qm = mx_codes_mem(q, M, H), sm = mx_scales_mem(s, M, H);
+  MW8_REQUIRE(!any_meet({rm, ym, qm, sm}, {wm}) && !any_meet({rm, qm, sm}, {xm}) && (y == x || !row_sets_meet(xm, ym)), kErrArg,
+              "rmsnorm_quant_mxfp4: residual, y (unless it is x), q and s must not overlap each other, x or weight");
   const bool ok = dispatch_rows<NormMxLaunch>(RowWork::kNormQuant, H / 8, M, st, static_cast<const uint16_t*>(x),
                                               static_cast<uint16_t*>(residual), static_cast<const uint16_t*>(weight),
                                               eps, M, H, q, s, static_cast<uint16_t*>(y));

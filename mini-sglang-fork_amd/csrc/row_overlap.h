@@ -1,4 +1,4 @@
-// Whether the rows of two tensors share memory (host).  A call that writes one
+// Whether the rows of tensors share memory (host).  A call that writes one
 // of them while other blocks read or write the other is refused.
 #pragma once
 
@@ -98,6 +98,19 @@ inline bool row_sets_meet(RowSet w, RowSet x) {
   for (int64_t i = 0; i < x.n_outer; ++i)
     for (int64_t j = 0; j < x.n_inner; ++j)
       if (row_meets(w, d + static_cast<wide_t>(i) * x.outer + static_cast<wide_t>(j) * x.inner, x.len)) return true;
+  return false;
+}
+
+// Whether any of `outs` shares a byte with another of them or one of `ins`
+// (one_row each).
+template <int NO, int NI>
+bool any_meet(const RowSet (&outs)[NO], const RowSet (&ins)[NI]) {
+  for (int i = 0; i < NO; ++i) {
+    for (int j = i + 1; j < NO; ++j)
+      if (row_sets_meet(outs[i], outs[j])) return true;
+    for (const RowSet& x : ins)
+      if (row_sets_meet(outs[i], x)) return true;
+  }
   return false;
 }
 

@@ -101,7 +101,8 @@ def rmsnorm_quant_mxfp4(
     """``rmsnorm_quant`` with the MXFP4 quantizer: bf16 x [M, H] -> (codes,
     scale[, bf16 y [M, H]]) of the normalized rows, bit-identical to
     ``quant_mxfp4`` of its y.  ``residual`` is added first and updated in
-    place; ``y`` may be ``x``, not ``residual``.  H % 8 == 0, H <= 32768."""
+    place; ``y`` may be ``x``; x, residual and y share no memory otherwise.
+    H % 8 == 0, H <= 32768."""
     _one_gpu(x, weight, residual, y)
     _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(), "x: bf16 [M, H] contiguous")
     M, H = x.shape
