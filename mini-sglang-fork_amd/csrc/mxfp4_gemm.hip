@@ -99,16 +99,11 @@ double mx_ring_us(int c, int64_t M, int64_t N, int64_t K, int split) {
   return us;
 }
 
-MxPlan mx_plan(int64_t M, int64_t N, int64_t K, bool may_split) {
-  may_split = may_split && N % 4 == 0;
+// The ring that the time model finds fastest, and its time.
+MxPlan mx_fastest_ring(int64_t M, int64_t N, int64_t K, bool may_split, double& us) {
   const int64_t tiles = mx_tiles(K);
-  if (g_mx_cfg >= 0) {
-    const bool split = may_split && g_mx_cfg == kMxSplitCfg && g_mx_split > 1 && g_mx_split <= tiles;
-    return {g_mx_cfg, split ? g_mx_split : 1};
-  }
-  if (M <= kMxDecodeRows || mx_shared_plan(M, N, K).waves > 0) return {-1, 1};
   MxPlan best{0, 1};
-  double us = 1e30;
+  us = 1e30;
   for (int c = 0; c < kNumMxRings; ++c) {
     const int most = may_split && c == kMxSplitCfg ? static_cast<int>(std::min<int64_t>(kMxMaxSplit, tiles)) : 1;
     for (int s = 1; s <= most; ++s) {
@@ -120,6 +115,17 @@ MxPlan mx_plan(int64_t M, int64_t N, int64_t K, bool may_split) {
     }
   }
   return best;
+}
+
+MxPlan mx_plan(int64_t M, int64_t N, int64_t K, bool may_split) {
+  may_split = may_split && N % 4 == 0;
+  if (g_mx_cfg >= 0) {
+    const bool split = may_split && g_mx_cfg == kMxSplitCfg && g_mx_split > 1 && g_mx_split <= mx_tiles(K);
+    return {g_mx_cfg, split ? g_mx_split : 1};
+  }
+  if (M <= kMxDecodeRows || mx_shared_plan(M, N, K).waves > 0) return {-1, 1};
+  double us;
+  return mx_fastest_ring(M, N, K, may_split, us);
 }
 
 template <int BM, int BN, int WM, int WN, int NS, bool kSplit = false, int kAct = -1>
@@ -280,14 +286,16 @@ int gemm_act_mxfp4_supported(int64_t M, int64_t I, int64_t K) {
 // product and act_and_mul_quant_mxfp4.  Fused: 6 us, and per round of 256-row x
 // 128-column tiles 3 us + 1.6 us a stage (MI355X, us, fused / two launches: 200 x
 // 25600 x 5120 49 / 69, 2080 rows 294 / 369; 333 x 17408 75 / 63, 2080 rows 193 /
-// 236; 1024 x 6400 39 / 49; K = 2048: 1024 x 768 18 / 13, 8192 rows 22 / 31).
+// 236; 1024 x 6400 39 / 49; K = 2048: 1024 x 768 18 / 13, 8192 rows 22 / 31).  Never
+// where the product would run on a decode kernel (17 rows: 32768 x 5120 45 / 32, 16384 x
+// 5120 35 / 19, 32768 x 512 11.7 / 10.2).
 int gemm_act_mxfp4_preferred(int64_t M, int64_t I, int64_t K) {
-  if (M <= kMxDecodeRows || !gemm_act_mxfp4_supported(M, I, K)) return 0;
+  if (M <= kMxDecodeRows || !gemm_act_mxfp4_supported(M, I, K) || mx_shared_plan(M, 2 * I, K).waves > 0) return 0;
   const int64_t cus = device_cus(), tiles = ((M + 255) / 256) * ((I + 127) / 128);
   const double rounds = static_cast<double>((tiles + cus - 1) / cus);
   const double fused = 6.0 + rounds * (3.0 + 1.6 * 2 * mx_tiles(K));
-  double us = 1e30;
-  for (int c = 0; c < kNumMxRings; ++c) us = std::min(us, mx_ring_us(c, M, 2 * I, K, 1));
+  double us;
+  mx_fastest_ring(M, 2 * I, K, true, us);
   return fused < us + 2.5 + 4.53 * M * I / 5.5e6;
 }
 
