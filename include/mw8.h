@@ -483,8 +483,11 @@ int32_t mw8_linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K);
 /*
  * The gate_up product, the gated activation and its quantizer in one launch:
  * W [2I, K] (gate rows, then up rows) -> q, s of bf16(act(gate) * up) [M, I],
- * gate and up rounded to bf16 first: bit-identical to mw8_gemm_mxfp4_bf16 +
- * mw8_act_and_mul_quant_mxfp4_bf16.  q 8-byte aligned.  _supported (host
+ * gate and up rounded to bf16 first: what mw8_gemm_mxfp4_bf16 +
+ * mw8_act_and_mul_quant_mxfp4_bf16 compute.  The bits are theirs where the fp32
+ * sums are exact; else the order of additions may differ (that product picks
+ * among kernels and K splits) and with it a last bit of gate or up.  q 8-byte
+ * aligned.  _supported (host
  * only): I % 32 == 0, I < 2^24, the codes of W below 2 GiB; _preferred: whether it is
  * also the faster way (larger batches).
  */
@@ -496,7 +499,8 @@ int32_t mw8_gemm_act_mxfp4_preferred(int64_t M, int64_t I, int64_t K);
 /*
  * The gated MLP: y bf16 [M, N] = down(act(gate) * up) with gate_up [2I, H] (gate
  * rows first) and down [N, I] quantized, of x bf16 [M, H] (row stride ldx) or,
- * if x is NULL, of quantized rows q, s; the bits of its parts one by one.
+ * if x is NULL, of quantized rows q, s; the bits of its parts one by one, where
+ * mw8_gemm_act_mxfp4_preferred says so with mw8_gemm_act_mxfp4 as one of them.
  * workspace: 16-byte aligned, at least _workspace_bytes(x == NULL, M, H, I, N) bytes
  * (the rows between the launches); calls that share one must be ordered on
  * one stream.  H, I <= 2^20.

@@ -206,8 +206,9 @@ def gemm_act_mxfp4(
     q: torch.Tensor, s_a: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, activation: str = "silu"
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes, scale) of act(gate) * up [M, I] for the quantized A [M, K] and
-    gate_up weight [2I, K]: one launch, the bits of ``gemm_mxfp4`` followed by
-    ``act_and_mul_quant_mxfp4``.  I % 32 == 0."""
+    gate_up weight [2I, K]: ``gemm_mxfp4`` and ``act_and_mul_quant_mxfp4`` in one
+    launch, with their bits but for the order of the product's fp32 additions
+    (``gemm_mxfp4`` picks among kernels and K splits).  I % 32 == 0."""
     _one_gpu(q, s_a, w, s_w)
     _need(activation in _ACT, f"unsupported activation {activation}")
     M, N = _check_operand("A", q, s_a, None), _check_operand("W", w, s_w, None)
