@@ -474,7 +474,8 @@ int32_t mw8_mxfp4_tuning_count(void);
  * The quantizer and the product of a decode batch in one launch: x bf16
  * [M, K] (row stride ldx, 16-byte aligned rows), bit-identical to
  * mw8_quant_mxfp4_bf16 + mw8_gemm_mxfp4_bf16.  _supported (host only): 1 if
- * it takes (M, N, K): up to 16 rows, K % 8 == 0, their codes fit a CU's LDS.
+ * it takes (M, N, K): K % 8 == 0 and few enough rows for a wave to quantize its
+ * part of K in 8 passes (8 rows at most, 2 at K = 5120), their codes in a CU's LDS.
  */
 int mw8_linear_bf16_mxfp4(const void* x, int64_t ldx, const uint8_t* W, const uint8_t* sw, const void* bias, void* y,
                           int64_t M, int64_t N, int64_t K, mw8_stream_t stream);

@@ -323,7 +323,7 @@ int gemm_act_mxfp4(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const 
 // 4 x 5120 -> 34816 21.6 us, in two launches 20.4, 2 rows 19.6 and 20.2), their
 // codes beside the weight ring in the LDS, K in whole 16-byte vectors.
 int linear_bf16_mxfp4_supported(int64_t M, int64_t N, int64_t K) {
-  if (M < 1 || M > kMxDecodeRows || N < 1 || N >= (1ll << 31) || K < 8 || K % 8 != 0 || K > (1ll << 20)) return 0;
+  if (M < 1 || M > kMxPasses || N < 1 || N >= (1ll << 31) || K < 8 || K % 8 != 0 || K > (1ll << 20)) return 0;
   const MxDecodePlan p = mx_decode_plan(M, N, K);
   return g_mx_cfg < 0 && M * p.per_wave <= (p.groups == 2 ? kMxPasses : kMxPasses / 2) &&
          mx_decode_lds(p, M, K, true) <= kLdsBytes;

@@ -231,8 +231,8 @@ def linear_mxfp4(
     x: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, bias: Optional[torch.Tensor] = None
 ) -> torch.Tensor:
     """bf16 x [..., K] times a quantized weight [N, K]: y bf16 [..., N].  The
-    rows of x are quantized (``quant_mxfp4``) on the way: up to 16 rows
-    inside the product's launch, with the same bits."""
+    rows of x are quantized (``quant_mxfp4``) on the way: a few rows (8 at
+    most, 2 at K = 5120) inside the product's launch, with the same bits."""
     _one_gpu(x, w, s_w, bias)
     _need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] > 0, "linear_mxfp4: x must be bf16 [..., K]")
     N = _check_operand("W", w, s_w, x.shape[-1])
@@ -242,7 +242,7 @@ def linear_mxfp4(
     _check_bias_out(bias, None, M, N)
     ldx = K if M <= 1 else x2.stride(0)
     # (the one launch reads x through a 32-bit view: rows less than 2^26 elements apart)
-    if 0 < M <= 16 and x2.data_ptr() % 16 == 0 and (M == 1 or (ldx % 8 == 0 and ldx < 1 << 26)):
+    if 0 < M <= 8 and x2.data_ptr() % 16 == 0 and (M == 1 or (ldx % 8 == 0 and ldx < 1 << 26)):
         lib = load()
         with _device_of(x):
             if lib.mw8_linear_bf16_mxfp4_supported(M, N, K):
