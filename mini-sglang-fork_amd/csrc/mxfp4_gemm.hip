@@ -1,7 +1,7 @@
 // MXFP4 products: y bf16 [M, N] = A W^T + bias of block-scaled 4-bit operands
-// (format: mxfp4.h).  Up to 16 tokens stream the weights once
-// (mxfp4_decode.h); more run on tile rings (mxfp4_ring.h), picked by a time
-// model.
+// (format: mxfp4.h).  Up to 16 tokens, on many weight rows 32, stream the
+// weights once (mxfp4_decode.h); more run on tile rings (mxfp4_ring.h), picked by
+// a time model.
 #include <algorithm>
 #include <atomic>
 
@@ -39,8 +39,9 @@ constexpr int kLdsBytes = 163840;
 // Tilings and what the time model knows of them (MI355X, fitted to graph-timed
 // runs of 130 random shapes from 17 to 8192 rows): us = start + (rounds - 1)
 // round + max(latency stages rounds, rate stages tiles per CU), at least
-// start + the operands and the output at bw TB/s.  On those shapes the pick is
-// 0.5% off the fastest configuration on average and 13% at most (78 x 51200 x 5120).
+// start + the operands and the output at bw TB/s.  On the shapes it was
+// fitted to the pick is 0.5% off the fastest configuration on average and 13% at
+// most (78 x 51200 x 5120).
 struct MxRingCfg {
   int bm, bn, per_cu;
   float start, round, latency, rate, bw;

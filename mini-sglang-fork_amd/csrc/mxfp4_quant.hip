@@ -4,8 +4,9 @@
 // one wave takes U rows of one 512-element tile (lane l holds elements
 // 8 l .. 8 l + 7, a quad of lanes holds a block), reads 1 KB and writes 256
 // code bytes per row, and the tile's 16 scale bytes.  Everything is read and
-// written once; the bound is HBM (MI355X: quantizer 8192 x 17408 59.6 us, 6.1
-// TB/s; dequantizer 53 us; activation + quantizer 110 us, 5.9 TB/s).
+// written once; the bound is HBM (MI355X, 8192 x 17408: quantizer 58-62 us, 5.9-6.2
+// TB/s; dequantizer 60-70 us, 5.2-6.0; silu + quantizer 105-112 us, 5.8-6.1; gelu +
+// quantizer 124-140 us, bound by the activation's instructions).
 #include "mxfp4.h"
 
 namespace mw8 {
@@ -126,7 +127,8 @@ int launch_quant(const char* what, const uint16_t* x, int64_t ldx, int64_t M, in
                  hipStream_t st) {
   const bool vec = K % 8 == 0 && (M == 1 || ldx % 8 == 0) && aligned_to(x, 16);
   // Four rows per wave once the chip is full of them: more loads in flight per
-  // wave (MI355X, us, one row / four: 2080 x 5120 8.0 / 7.4, 64 x 17408 3.0 / 4.4).
+  // wave (MI355X, us, one row / four: 2080 x 5120 7.3 / 6.6, 8192 x 17408 67 / 58, but
+  // 64 x 17408 3.0 / 4.4).
   const int U = M * mx_tiles(K) >= 16384 ? 4 : 1;
   const unsigned grid = mx_grid(M, K, U);
   MW8_REQUIRE(grid > 0, kErrShape, "%s: M=%lld x K=%lld too large", what, (long long)M, (long long)K);

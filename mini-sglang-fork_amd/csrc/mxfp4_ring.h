@@ -12,8 +12,8 @@
 // beside 256 matrix cycles per SIMD pair; one block per CU walks its tiles, the
 // first stages of the next one in flight during the epilogue; the weight rows
 // are the instruction's rows, so that a lane holds 4 adjacent columns and the
-// epilogue packs and stores from registers.  MI355X: 8192 x 34816 x 5120 716-735
-// us (4.0-4.1 PFLOP/s), 8192 x 5120 x 17408 332 us (4.4).  What bounds it: without
+// epilogue packs and stores from registers.  MI355X: 8192 x 34816 x 5120 691-735
+// us (4.0-4.2 PFLOP/s), 8192 x 5120 x 17408 332 us (4.4).  What bounds it: without
 // the DMA the first takes 556 us, with the DMA's lines in the L2 666 (a stage's
 // loads have one stage to arrive; the LDS has no room for a third slot), and
 // the output's stores the rest.
