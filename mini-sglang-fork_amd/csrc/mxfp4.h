@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t mx_quad_max(uint32_t m) {
 // a^2 is exact (g holds a bf16 value) and h(a) = t Q(t) with t = 1 / (1 + 0.3 a): Q is
 // the polynomial of degree 7 with the least relative error on 0 <= a <= 13.5 (2^-22.9;
 // past it the product leaves fp32's range).  MI355X, 8192 x 17408 activations:
-// 129 us; with erfcf 215, with 1 + erff 166; silu 105.
+// 130 us; with erfcf 215, with 1 + erff 166; silu 105.
 template <int ACT>
 __device__ __forceinline__ float mx_act_fn(float g) {
   // silu: to zero from g = -87.3 down (below 2^-119; the reciprocal of e^87.3 is
@@ -110,7 +110,7 @@ __device__ __forceinline__ float mx_act_fn(float g) {
   q = __builtin_fmaf(q, t, 0.120798387f);
   q = __builtin_fmaf(q, t, 0.119626388f);
   const float e = __builtin_amdgcn_exp2f(g * g * -0.72134752044448170368f);  // / (2 ln 2)
-  return __builtin_fmaxf(g, 0.0f) - a * t * (q * e);
+  return __builtin_fmaxf(g, -0.0f) - a * t * (q * e);  // (-0: a zero keeps g's sign)
 }
 
 // Quantizes the block of which this lane of a quad holds 8 elements; every

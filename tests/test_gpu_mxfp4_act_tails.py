@@ -71,6 +71,21 @@ def test_silu_tail():
     _check(x, "silu", (np.abs(f32(x).astype(np.float64)[:, :256]) + 8) * 2.0**-23)
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_zeros_keep_their_sign(act):
+    """Gates of zero, and ones so low that the activation underflows, beside one
+    that sets the block's scale: codes 0 and 8 by the oracle's signs."""
+    announce(f"act_and_mul_quant_mxfp4 signed zeros {act}")
+    gates = torch.tensor([1.0, 0.0, -0.0, -30.0, -200.0, -1e-40, 1e-40, -3e38] * 4)
+    for up in (2.0, -2.0, 0.0, -0.0):
+        x = torch.cat([gates, torch.full((32,), up)]).bfloat16()[None]
+        codes, scale = act_and_mul_quant_mxfp4(x.to(DEV), act)
+        xv = f32(x).astype(np.float64)
+        code, byte = orc.quantize(orc.round_bf16(orc.activation(xv[:, :32], act) * xv[:, 32:]))
+        np.testing.assert_array_equal(codes.cpu().numpy(), orc.pack(code))
+        np.testing.assert_array_equal(mxfp4_row_scales(scale, 32).cpu().numpy(), byte)
+
+
 def _rows_of_gates(count, value, N, seed):
     """Quantized A [M, 64] of ones in the first count[m] columns, zeros behind,
     and W [2 N, 64]: gate rows `value`, up rows random levels.  So the gates of
